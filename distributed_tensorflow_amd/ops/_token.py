@@ -1,0 +1,46 @@
+"""What the token-model operators (``layernorm``, ``dropout``, ``embedding``, ``vocab_xent``) share: operand checks and
+the launch on a tensor's own device and stream.
+
+Workspaces come from PyTorch's allocator call by call: each belongs to the stream the call runs on, and to the graph
+that captured it, so neither two streams nor two graphs ever share one.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1}       # element type codes of the C entry points
+
+
+def dtype_code(t: torch.Tensor, what: str) -> int:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
+    return code
+
+
+def same_device(what: str, first: torch.Tensor, *others) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on different devices: {first.device} vs {t.device}")
+
+
+def rows_2d(t: torch.Tensor, cols: int):
+    """``t`` as rows of ``cols`` elements and the distance between them; a copy only where no such view exists."""
+    r = t.reshape(-1, cols)
+    ld = r.stride(0) if r.shape[0] > 1 else cols
+    if (cols > 1 and r.stride(1) != 1) or ld < cols:
+        r, ld = r.contiguous(), cols
+    return r, ld
+
+
+def launch(what: str, fn, t: torch.Tensor, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``t``'s device, whatever the current device is."""
+    if t.device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(t.device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc, what)

@@ -132,3 +132,62 @@ def softmax_xent(logits, labels, loss_mode=LOSS_STANDARD, grad_scale=None):
         logp = torch.log_softmax(z, 1)
         dz = (y - lab) * scale
     return {"loss_rows": -(lab * logp).sum(1), "dlogits": dz, "correct": int((z.argmax(1) == am_l).sum().item())}
+
+
+# ------------------------------------------------------------------------------------------- token-model operators
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """``(y, h, mean, rstd)`` of layer normalisation over the last axis of ``h = x [+ residual]`` (``h`` as stored)."""
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    v = h.float()
+    mean = v.mean(-1, keepdim=True)
+    centred = v - mean
+    rstd = torch.rsqrt((centred * centred).mean(-1, keepdim=True) + eps)
+    y = centred * rstd
+    if weight is not None:
+        y = y * weight.float()
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(x.dtype), h, mean.reshape(-1), rstd.reshape(-1)
+
+
+def layer_norm_bwd(dy, h, mean, rstd, weight=None, dh=None):
+    """``(dx, dweight, dbias)``; the parameters' gradients in float32."""
+    cols = h.shape[-1]
+    d = dy.float().reshape(-1, cols)
+    xhat = (h.float().reshape(-1, cols) - mean[:, None]) * rstd[:, None]
+    g = d if weight is None else d * weight.float()
+    dx = rstd[:, None] * (g - g.mean(1, keepdim=True) - xhat * (g * xhat).mean(1, keepdim=True))
+    if dh is not None:
+        dx = dx + dh.float().reshape(-1, cols)
+    return dx.to(h.dtype).reshape(dy.shape), (d * xhat).sum(0), d.sum(0)
+
+
+def philox_words(blocks, seed, step, device="cpu"):
+    """``[blocks, 4]`` words (int64 holding 32 bits) of Philox4x32-10 for the counters ``(i, step)`` under key ``seed``."""
+    m32 = 0xFFFFFFFF
+    i = torch.arange(blocks, dtype=torch.int64, device=device)
+    c = [i & m32, i >> 32, torch.full_like(i, step & m32), torch.full_like(i, (step >> 32) & m32)]
+    k0, k1 = seed & m32, (seed >> 32) & m32
+    for _ in range(10):
+        p0, p1 = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57          # modulo 2^64: the sign bit is a bit like the others
+        c = [((p1 >> 32) & m32) ^ c[1] ^ k0, p1 & m32, ((p0 >> 32) & m32) ^ c[3] ^ k1, p0 & m32]
+        k0, k1 = (k0 + 0x9E3779B9) & m32, (k1 + 0xBB67AE85) & m32
+    return torch.stack(c, 1)
+
+
+def dropout_mask(shape, rate, seed, step, device="cpu"):
+    """True where dropout keeps the element: its 16-bit number is at least ``round(rate * 65536)``."""
+    n = math.prod(shape)
+    w = philox_words(-(-n // 8), seed, step, device)
+    u = torch.stack((w & 0xFFFF, w >> 16), 2).reshape(-1)[:n]
+    return (u >= int(round(rate * 65536))).reshape(shape)
+
+
+def dropout(x, rate, seed, step=0, residual=None):
+    thr = int(round(rate * 65536))
+    scale = 65536.0 / (65536 - thr) if thr < 65536 else 0.0
+    kept = dropout_mask(tuple(x.shape), rate, seed, step, x.device)
+    y = torch.where(kept, x.float() * scale, torch.zeros((), dtype=torch.float32, device=x.device))
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(x.dtype)
