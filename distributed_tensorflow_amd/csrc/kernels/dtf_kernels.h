@@ -511,3 +511,29 @@ DTF_EXPORT int dtf_truncated_normal(float* out, int64_t n, float stddev, uint64_
 DTF_EXPORT int dtf_accumulate(float* dst, const float* src, int64_t n, float alpha, float beta, hipStream_t s);
 DTF_EXPORT int dtf_upload_words(void* dst, const void* host_src, int64_t n_words, hipStream_t s);
 DTF_EXPORT int dtf_kernels_abi_version();
+
+// Softmax cross entropy over a large vocabulary in pieces (vocab_xent.hip).  Forward reads X, W, labels, bias and writes
+// lse, loss_rows, loss, counts; backward reads those, and dloss, and writes dX [N, D], dW [V, D], dbias [V] (dense; null:
+// left out).
+struct DtfVocabXentArgs {
+  const void* X;            // [N, ldx] of `dtype`
+  const void* W;            // [V, ldw] of `w_dtype`: `dtype`, or fp32 under bf16 activations
+  const float* bias;        // [V], optional
+  const long long* labels;  // [N] class indices; `ignore`: a row without loss
+  float* lse;               // [N]
+  float* loss_rows;         // [N]
+  float* loss;              // [1] mean over the rows with a label, or sum
+  long long* counts;        // [2] hits, rows with a label
+  const float* dloss;       // [1] or [N] (dloss_rows); null: 1
+  void* dX;
+  void* dW;
+  float* dbias;
+  void* ws;                 // dtf_vocab_xent_ws_bytes, 16-byte aligned
+  int64_t ws_bytes;
+  long long ignore;
+  int64_t ldx, ldw;
+  int64_t V;
+  int N, D;
+  int dtype, w_dtype;       // 0 fp32, 1 bf16
+  int mean, dloss_rows;
+};

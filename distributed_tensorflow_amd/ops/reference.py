@@ -191,3 +191,44 @@ def dropout(x, rate, seed, step=0, residual=None):
     if residual is not None:
         y = y + residual.float()
     return y.to(x.dtype)
+
+
+def _vocab_labels(labels, vocab, ignore_index):
+    valid = labels != ignore_index
+    lab = torch.where(valid, labels, torch.zeros_like(labels))
+    if bool(((lab < 0) | (lab >= vocab)).any()):
+        raise IndexError(f"vocab_xent: a label lies outside [0, {vocab}) and is not ignore_index")
+    return valid, lab
+
+
+def vocab_xent(features, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
+    """``(loss, loss_rows, lse, [hits, rows with a label])`` of softmax cross entropy on ``features @ weight.T + bias``."""
+    z = features.float() @ weight.float().t()
+    if bias is not None:
+        z = z + bias.float()
+    valid, lab = _vocab_labels(labels, weight.shape[0], ignore_index)
+    lse = torch.logsumexp(z, 1)
+    rows = torch.where(valid, lse - z.gather(1, lab[:, None])[:, 0], torch.zeros_like(lse))
+    counts = torch.stack([((z.argmax(1) == lab) & valid).sum(), valid.sum()])
+    total = rows.sum()
+    if reduction == "mean":
+        total = total / counts[1].clamp_min(1)
+    return total, rows, lse, counts
+
+
+def vocab_xent_bwd(features, weight, labels, bias, lse, counts, ignore_index=-100, reduction="mean", dloss=None):
+    """``(dfeatures, dweight, dbias)``; dbias None without a bias."""
+    x, w = features.float(), weight.float()
+    z = x @ w.t()
+    if bias is not None:
+        z = z + bias.float()
+    valid, lab = _vocab_labels(labels, weight.shape[0], ignore_index)
+    g = torch.ones((), device=x.device) if dloss is None else dloss.float().reshape(-1 if reduction == "none" else ())
+    if reduction == "mean":
+        g = g / counts[1].clamp_min(1)
+    g = torch.where(valid, g.expand(x.shape[0]), torch.zeros((), device=x.device))
+    dz = torch.exp(z - lse[:, None])
+    dz.scatter_add_(1, lab[:, None], torch.full_like(lse, -1.0)[:, None])
+    dz = dz * g[:, None]
+    db = None if bias is None else dz.sum(0).to(bias.dtype)
+    return (dz @ w).to(features.dtype), (dz.t() @ x).to(weight.dtype), db
