@@ -232,3 +232,16 @@ def vocab_xent_bwd(features, weight, labels, bias, lse, counts, ignore_index=-10
     dz = dz * g[:, None]
     db = None if bias is None else dz.sum(0).to(bias.dtype)
     return (dz @ w).to(features.dtype), (dz.t() @ x).to(weight.dtype), db
+
+
+def embedding(ids, table, scale=1.0):
+    return (torch.nn.functional.embedding(ids.long(), table).float() * scale).to(table.dtype)
+
+
+def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=None):
+    flat, d = ids.reshape(-1).long(), dy.float().reshape(-1, dy.shape[-1])
+    if padding_idx is not None:
+        keep = flat != padding_idx % rows
+        flat, d = flat[keep], d[keep]
+    out = torch.zeros((rows, dy.shape[-1]), dtype=torch.float32, device=dy.device)
+    return (out.index_add_(0, flat, d) * scale).to(dy.dtype)
