@@ -9,12 +9,14 @@
 // sum of squares minus the squared mean would cancel for rows whose mean is large against their spread.
 //
 // Layout.  A row belongs to TPR threads (one wave up to a whole workgroup) and is read ONCE into registers with 16-byte
-// accesses (8 bf16 / 4 fp32; single elements where width, stride or address do not allow them).  TPR is the smallest of
-// 64 / 256 / 512 / 1024 for which a thread holds at most 16 elements: in the backward pass a thread keeps its columns'
-// running dw and db, the weight, xhat and g in registers, five floats an element.  The backward pass runs on at most
-// 256 workgroups of 1024 threads, each walking over rows and leaving ONE partial [dw | db] (so the partials stay a few
-// per cent of the traffic); a second launch adds the partials in workgroup order.  No atomics: the same inputs give the
-// same bits.  Rows too wide for registers are streamed (three passes forward, two backward, column sums on their own).
+// accesses (8 bf16 / 4 fp32; at the elements' own alignment where width, stride or address ask for it).  TPR is the smallest
+// of 64 / 256 / 512 / 1024 for which a thread holds at most 16 elements (backward: 32 past 8192 columns): in the backward
+// pass a thread keeps its columns' running dw and db, the weight, xhat and g in registers, five floats an element.  The
+// backward pass runs on at most 256 workgroups of 512 threads, each walking over rows and leaving ONE partial [dw | db] (so
+// the partials stay a few per cent of the traffic); while a row's sums cross the workgroup, the next row is already on its
+// way: 8 waves a CU with 96 bytes a lane in flight cover the latency at full bandwidth.  A second launch adds the partials
+// in workgroup order.  No atomics: the same inputs give the same bits.  Rows too wide for registers are streamed
+// (three passes forward, two backward, column sums on their own).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,6 +25,7 @@
 
 namespace {
 constexpr int kBlock = 1024;
+constexpr int kBwdBlock = 512;               // 256 registers a thread: the backward pass keeps a row, its gradients and the next row
 constexpr int kMaxParts = 256;               // workgroups of the backward pass, one per CU
 
 struct LnArgs {
@@ -59,56 +62,62 @@ __device__ __forceinline__ void row_sum(float (&v)[NVAL], float (*s)[NVAL][kBloc
   }
 }
 
-template <typename T, int VEC, int NV, int TPR, int BLOCK>
+template <typename T, bool AL, int NV, int TPR, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LnArgs a) {
+  typedef TkPiece<T, AL> P;
+  constexpr int VEC = P::VEC;
   __shared__ float s_sum[2][1][kBlock / 64];
   const int t = threadIdx.x % TPR;
   const long row = (long)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
   const bool live = row < a.rows;            // dead rows of the last workgroup still take part in its barriers
   const T* const x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
+  tk_u32x4 raw[NV];
   float v[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * TPR + t) * VEC;
-    if (live && c < a.C) {
-      TkVec<T, VEC>::load(x + c, v[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = 0.f;
-    }
+    raw[j] = live && c < a.C ? P::load(x, c, a.C) : tk_u32x4{0u, 0u, 0u, 0u};
   }
   if (a.res) {
     const T* const r = static_cast<const T*>(a.res) + (live ? row : 0) * a.ldres;
     T* const h = static_cast<T*>(a.h) + row * a.C;
+    tk_u32x4 rr[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * TPR + t) * VEC;
-      if (live && c < a.C) {
-        float q[VEC];
-        TkVec<T, VEC>::load(r + c, q);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = tk_round(h, v[j][i] + q[i]);       // normalised as the stream stores it
-        TkVec<T, VEC>::store(h + c, v[j]);
-      }
+      rr[j] = live && c < a.C ? P::load(r, c, a.C) : tk_u32x4{0u, 0u, 0u, 0u};
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * VEC;
+      float q[VEC];
+      P::unpack(raw[j], v[j]);
+      P::unpack(rr[j], q);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j][i] = tk_round(h, v[j][i] + q[i]);         // normalised as the stream stores it
+      if (live && c < a.C) P::store(h, c, a.C, v[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) P::unpack(raw[j], v[j]);
   }
   int half = 0;
   float s[1] = {0.f};
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s[0] += v[j][i];
+    for (int i = 0; i < VEC; ++i) s[0] += v[j][i];           // zeros past the row's end
   row_sum<TPR, 1>(s, s_sum, half);
   const float inv_c = 1.f / (float)a.C;
   const float mean = s[0] * inv_c;
   s[0] = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const bool in = (j * TPR + t) * VEC < a.C;
+    const int c = (j * TPR + t) * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       v[j][i] -= mean;
-      if (in) s[0] = fmaf(v[j][i], v[j][i], s[0]);
+      if (AL ? c < a.C : c + i < a.C) s[0] = fmaf(v[j][i], v[j][i], s[0]);
     }
   }
   row_sum<TPR, 1>(s, s_sum, half);
@@ -126,11 +135,11 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LnArgs a) {
       float w[VEC], b[VEC], o[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { w[i] = 1.f; b[i] = 0.f; }
-      if (a.w) tk_load_param<VEC>(a.w, a.w_bf16, c, w);
-      if (a.b) tk_load_param<VEC>(a.b, a.w_bf16, c, b);
+      if (a.w) tk_load_param<VEC>(a.w, a.w_bf16, c, AL ? 0x7fffffff : a.C, 1.f, w);
+      if (a.b) tk_load_param<VEC>(a.b, a.w_bf16, c, AL ? 0x7fffffff : a.C, 0.f, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) o[i] = fmaf(v[j][i] * rstd, w[i], b[i]);
-      TkVec<T, VEC>::store(y + c, o);
+      P::store(y, c, a.C, o);
     }
   }
 }
@@ -170,15 +179,17 @@ __global__ __launch_bounds__(kBlock) void ln_fwd_stream_kernel(LnArgs a) {
   T* const y = static_cast<T*>(a.y) + row * a.C;
   for (int c = threadIdx.x; c < a.C; c += kBlock) {
     float w[1] = {1.f}, b[1] = {0.f};
-    if (a.w) tk_load_param<1>(a.w, a.w_bf16, c, w);
-    if (a.b) tk_load_param<1>(a.b, a.w_bf16, c, b);
+    if (a.w) tk_load_param<1>(a.w, a.w_bf16, c, a.C, 1.f, w);
+    if (a.b) tk_load_param<1>(a.b, a.w_bf16, c, a.C, 0.f, b);
     tk_put(y + c, fmaf((tk_get(src + c) - mean) * rstd, w[0], b[0]));
   }
 }
 
-template <typename T, int VEC, int NV, int TPR>
-__global__ __launch_bounds__(kBlock) void ln_bwd_kernel(LnBwdArgs a) {
-  constexpr int RPB = kBlock / TPR, COLS = NV * TPR * VEC;
+template <typename T, bool AL, int NV, int TPR>
+__global__ __launch_bounds__(kBwdBlock) void ln_bwd_kernel(LnBwdArgs a) {
+  typedef TkPiece<T, AL> P;
+  constexpr int VEC = P::VEC, RPB = kBwdBlock / TPR, COLS = NV * TPR * VEC;
+  constexpr bool AHEAD = NV * VEC <= 16;     // the next row's pieces fit the registers
   __shared__ float s_sum[2][2][kBlock / 64];
   __shared__ float s_col[RPB > 1 ? COLS : 1];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -188,42 +199,65 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_kernel(LnBwdArgs a) {
     const int c = (j * TPR + t) * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { w[j][i] = 1.f; aw[j][i] = 0.f; ab[j][i] = 0.f; }
-    if (a.w && c < a.C) tk_load_param<VEC>(a.w, a.w_bf16, c, w[j]);
+    if (a.w && c < a.C) tk_load_param<VEC>(a.w, a.w_bf16, c, AL ? 0x7fffffff : a.C, 0.f, w[j]);
   }
   const float inv_c = 1.f / (float)a.C;
   int half = 0;
   const long step = (long)gridDim.x * RPB;
+  // what a row brings: dy and h as loaded, its statistics; zeros past the row's end and for rows that do not exist
+  tk_u32x4 ndy[NV], nh[NV];
+  float nmean, nrstd;
+  auto fetch = [&](long row) {
+    const bool live = row < a.rows;
+    const T* const dy = static_cast<const T*>(a.dy) + (live ? row : 0) * a.lddy;
+    const T* const h = static_cast<const T*>(a.h) + (live ? row : 0) * a.ldh;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + t) * VEC;
+      const bool in = live && c < a.C;
+      nh[j] = in ? P::load(h, c, a.C) : tk_u32x4{0u, 0u, 0u, 0u};
+      ndy[j] = in ? P::load(dy, c, a.C) : tk_u32x4{0u, 0u, 0u, 0u};
+    }
+    nmean = live ? a.mean[row] : 0.f;
+    nrstd = live ? a.rstd[row] : 0.f;
+  };
+  if (AHEAD) fetch((long)blockIdx.x * RPB + sub);
   for (long row0 = (long)blockIdx.x * RPB; row0 < a.rows; row0 += step) {      // the same count for every wave
     const long row = row0 + sub;
     const bool live = row < a.rows;
-    const long rr = live ? row : 0;
-    const T* const dy = static_cast<const T*>(a.dy) + rr * a.lddy;
-    const T* const h = static_cast<const T*>(a.h) + rr * a.ldh;
-    const float mean = a.mean[rr], rstd = a.rstd[rr];
+    if (!AHEAD) fetch(row);
+    const float mean = nmean, rstd = nrstd;
     float xh[NV][VEC], g[NV][VEC];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * TPR + t) * VEC;
-      if (live && c < a.C) {
-        TkVec<T, VEC>::load(h + c, xh[j]);
-        TkVec<T, VEC>::load(dy + c, g[j]);
+      P::unpack(nh[j], xh[j]);
+      P::unpack(ndy[j], g[j]);                 // dy = 0 past the row's end: no share in any sum, whatever xh is there
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          xh[j][i] = (xh[j][i] - mean) * rstd;
-          aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
-          ab[j][i] += g[j][i];
-          g[j][i] *= w[j][i];
-          s[0] += g[j][i];
-          s[1] = fmaf(g[j][i], xh[j][i], s[1]);
-        }
+      for (int i = 0; i < VEC; ++i) {
+        xh[j][i] = (xh[j][i] - mean) * rstd;
+        if (!AL && c + i >= a.C) xh[j][i] = 0.f;
+        aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
+        ab[j][i] += g[j][i];
+        g[j][i] *= w[j][i];
+        s[0] += g[j][i];
+        s[1] = fmaf(g[j][i], xh[j][i], s[1]);
+      }
+    }
+    if (AHEAD) fetch(row + step);              // on its way while the sums below cross the workgroup
+    tk_u32x4 q[NV];
+    if (a.dh) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * VEC;
+        q[j] = live && c < a.C ? P::load(static_cast<const T*>(a.dh) + row * a.lddh, c, a.C) : tk_u32x4{0u, 0u, 0u, 0u};
       }
     }
     row_sum<TPR, 2>(s, s_sum, half);
     const float m1 = s[0] * inv_c, m2 = s[1] * inv_c;
     if (live) {
       T* const dx = static_cast<T*>(a.dx) + row * a.C;
-      const T* const dh = a.dh ? static_cast<const T*>(a.dh) + row * a.lddh : nullptr;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = (j * TPR + t) * VEC;
@@ -231,13 +265,13 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_kernel(LnBwdArgs a) {
           float o[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) o[i] = rstd * (g[j][i] - fmaf(xh[j][i], m2, m1));
-          if (dh) {
-            float q[VEC];
-            TkVec<T, VEC>::load(dh + c, q);
+          if (a.dh) {
+            float z[VEC];
+            P::unpack(q[j], z);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] += q[i];
+            for (int i = 0; i < VEC; ++i) o[i] += z[i];
           }
-          TkVec<T, VEC>::store(dx + c, o);
+          P::store(dx, c, a.C, o);
         }
       }
     }
@@ -278,7 +312,7 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_stream_kernel(LnBwdArgs a) {
   float s[2] = {0.f, 0.f};
   for (int c = threadIdx.x; c < a.C; c += kBlock) {
     float w[1] = {1.f};
-    if (a.w) tk_load_param<1>(a.w, a.w_bf16, c, w);
+    if (a.w) tk_load_param<1>(a.w, a.w_bf16, c, a.C, 1.f, w);
     const float g = tk_get(dy + c) * w[0];
     s[0] += g;
     s[1] = fmaf(g, (tk_get(h + c) - mean) * rstd, s[1]);
@@ -287,7 +321,7 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_stream_kernel(LnBwdArgs a) {
   const float m1 = s[0] * inv_c, m2 = s[1] * inv_c;
   for (int c = threadIdx.x; c < a.C; c += kBlock) {
     float w[1] = {1.f};
-    if (a.w) tk_load_param<1>(a.w, a.w_bf16, c, w);
+    if (a.w) tk_load_param<1>(a.w, a.w_bf16, c, a.C, 1.f, w);
     float o = rstd * (tk_get(dy + c) * w[0] - fmaf((tk_get(h + c) - mean) * rstd, m2, m1));
     if (dh) o += tk_get(dh + c);
     tk_put(dx + c, o);
@@ -333,43 +367,41 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
 
 bool vec_ok(const void* p, long ld, int vec, int es) { return !p || (((uintptr_t)p & 15) == 0 && ld % vec == 0 && vec * es == 16); }
 
-template <typename T, int VEC, int NV, int TPR>
+template <typename T, bool AL, int NV, int TPR>
 void fwd_as(const LnArgs& a, hipStream_t s) {
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   const long rpb = BLOCK / TPR;
-  hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, NV, TPR, BLOCK>), dim3((unsigned)((a.rows + rpb - 1) / rpb)), dim3(BLOCK), 0, s, a);
+  hipLaunchKernelGGL((ln_fwd_kernel<T, AL, NV, TPR, BLOCK>), dim3((unsigned)((a.rows + rpb - 1) / rpb)), dim3(BLOCK), 0, s, a);
 }
 
-template <typename T, int VEC>
+template <typename T, bool AL>
 void fwd_width(const LnArgs& a, hipStream_t s) {
-  constexpr int N16 = 16 / VEC;              // vectors a thread for 16 elements
-  if (a.C <= 64 * VEC) fwd_as<T, VEC, 1, 64>(a, s);
-  else if (a.C <= 64 * 16) fwd_as<T, VEC, N16, 64>(a, s);
-  else if (a.C <= 256 * 16) fwd_as<T, VEC, N16, 256>(a, s);
-  else if (a.C <= 512 * 16) fwd_as<T, VEC, N16, 512>(a, s);
-  else if (a.C <= 1024 * 16) fwd_as<T, VEC, N16, 1024>(a, s);
+  constexpr int VEC = TkPiece<T, AL>::VEC, N16 = 16 / VEC;              // N16 pieces a thread: 16 elements
+  if (a.C <= 64 * VEC) fwd_as<T, AL, 1, 64>(a, s);
+  else if (a.C <= 64 * 16) fwd_as<T, AL, N16, 64>(a, s);
+  else if (a.C <= 256 * 16) fwd_as<T, AL, N16, 256>(a, s);
+  else if (a.C <= 512 * 16) fwd_as<T, AL, N16, 512>(a, s);
+  else if (a.C <= 1024 * 16) fwd_as<T, AL, N16, 1024>(a, s);
   else hipLaunchKernelGGL((ln_fwd_stream_kernel<T>), dim3((unsigned)a.rows), dim3(kBlock), 0, s, a);
 }
 
-template <typename T>
-int bwd_parts(const LnBwdArgs& a) {
-  if (a.C > 1024 * 16) return (int)std::min<long>(std::max<long>(1, a.rows / 64), 64);
-  const int tpr = a.C <= 64 * 16 ? 64 : a.C <= 256 * 16 ? 256 : a.C <= 512 * 16 ? 512 : 1024;
-  const long rpb = kBlock / tpr;
-  return (int)std::min<long>((a.rows + rpb - 1) / rpb, kMaxParts);
+int bwd_parts(long rows, int C) {
+  if (C > 1024 * 16) return (int)std::min<long>(std::max<long>(1, rows / 64), 64);
+  const long rpb = kBwdBlock / (C <= 64 * 16 ? 64 : C <= 256 * 16 ? 256 : 512);
+  return (int)std::min<long>((rows + rpb - 1) / rpb, kMaxParts);
 }
 
-template <typename T, int VEC>
+template <typename T, bool AL>
 void bwd_width(const LnBwdArgs& a, int parts, hipStream_t s) {
-  constexpr int N16 = 16 / VEC;
-  const dim3 g(parts), b(kBlock);
-  if (a.C <= 64 * VEC) hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, 1, 64>), g, b, 0, s, a);
-  else if (a.C <= 64 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, N16, 64>), g, b, 0, s, a);
-  else if (a.C <= 256 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, N16, 256>), g, b, 0, s, a);
-  else if (a.C <= 512 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, N16, 512>), g, b, 0, s, a);
-  else if (a.C <= 1024 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, N16, 1024>), g, b, 0, s, a);
+  constexpr int VEC = TkPiece<T, AL>::VEC, N16 = 16 / VEC;
+  const dim3 g(parts), b(kBwdBlock);
+  if (a.C <= 64 * VEC) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, 1, 64>), g, b, 0, s, a);
+  else if (a.C <= 64 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, N16, 64>), g, b, 0, s, a);
+  else if (a.C <= 256 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, N16, 256>), g, b, 0, s, a);
+  else if (a.C <= 512 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, N16, 512>), g, b, 0, s, a);
+  else if (a.C <= 1024 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, 2 * N16, 512>), g, b, 0, s, a);
   else {
-    hipLaunchKernelGGL((ln_bwd_stream_kernel<T>), dim3((unsigned)a.rows), b, 0, s, a);
+    hipLaunchKernelGGL((ln_bwd_stream_kernel<T>), dim3((unsigned)a.rows), dim3(kBlock), 0, s, a);
     if (a.want_wgrad) hipLaunchKernelGGL((ln_colsum_kernel<T>), dim3(dtf_cdiv(a.C, 256), parts), dim3(256), 0, s, a);
   }
 }
@@ -386,18 +418,14 @@ DTF_EXPORT int dtf_layernorm_fwd(const void* x, const void* res, const void* w, 
   const LnArgs a = {x, res, w, b, y, h, mean, rstd, (long)rows, C, (long)ldx, (long)ldres, w_dtype, eps};
   const int es = dtype == TK_BF16 ? 2 : 4, vec = 16 / es;
   const bool v = C % vec == 0 && vec_ok(x, ldx, vec, es) && vec_ok(res, ldres, vec, es) && vec_ok(y, C, vec, es) && vec_ok(h, C, vec, es);
-  if (dtype == TK_BF16) v ? fwd_width<unsigned short, 8>(a, s) : fwd_width<unsigned short, 1>(a, s);
-  else v ? fwd_width<float, 4>(a, s) : fwd_width<float, 1>(a, s);
+  if (dtype == TK_BF16) v ? fwd_width<unsigned short, true>(a, s) : fwd_width<unsigned short, false>(a, s);
+  else v ? fwd_width<float, true>(a, s) : fwd_width<float, false>(a, s);
   return dtf_check_launch();
 }
 
 // Floats of the workspace `part` that the backward pass needs.
 DTF_EXPORT int64_t dtf_layernorm_bwd_ws_floats(int64_t rows, int C) {
-  if (rows <= 0 || C <= 0) return 0;
-  LnBwdArgs a = {};
-  a.rows = (long)rows;
-  a.C = C;
-  return (int64_t)bwd_parts<float>(a) * 2 * C;
+  return rows <= 0 || C <= 0 ? 0 : (int64_t)bwd_parts((long)rows, C) * 2 * C;
 }
 
 // dw, db (dtype w_dtype): null to leave one out; part only if one of them is wanted.
@@ -411,11 +439,11 @@ DTF_EXPORT int dtf_layernorm_bwd(const void* dy, const void* h, const void* dh, 
   int parts = 0;
   if (rows > 0) {
     if (!dy || !h || !mean || !rstd || !dx || (wgrad && !part)) return DTF_ERR_ARG;
-    parts = bwd_parts<float>(a);
+    parts = bwd_parts((long)rows, C);
     const int es = dtype == TK_BF16 ? 2 : 4, vec = 16 / es;
     const bool v = C % vec == 0 && vec_ok(dy, lddy, vec, es) && vec_ok(h, ldh, vec, es) && vec_ok(dh, lddh, vec, es) && vec_ok(dx, C, vec, es);
-    if (dtype == TK_BF16) v ? bwd_width<unsigned short, 8>(a, parts, s) : bwd_width<unsigned short, 1>(a, parts, s);
-    else v ? bwd_width<float, 4>(a, parts, s) : bwd_width<float, 1>(a, parts, s);
+    if (dtype == TK_BF16) v ? bwd_width<unsigned short, true>(a, parts, s) : bwd_width<unsigned short, false>(a, parts, s);
+    else v ? bwd_width<float, true>(a, parts, s) : bwd_width<float, false>(a, parts, s);
   }
   if (wgrad)
     hipLaunchKernelGGL(ln_join_kernel, dim3(dtf_cdiv(C, 64), 2), dim3(1024), 0, s, part, parts, C, dw, db, w_dtype);

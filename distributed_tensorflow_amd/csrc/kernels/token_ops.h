@@ -44,16 +44,61 @@ template <> struct TkVec<float, 4> {
   }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
 };
+// A row piece of VEC elements at column c of a row of C, as the 16 bytes that a lane holds: ALIGNED where every piece is
+// whole and 16-byte aligned, else by one 16-byte access at the elements' own alignment (the hardware splits it where it
+// crosses a line) and element by element in the row's last piece.
+typedef tk_u32x4 tk_u32x4_at2 __attribute__((aligned(2)));
+template <typename T, bool ALIGNED>
+struct TkPiece {
+  static constexpr int VEC = 16 / sizeof(T);
+  static __device__ __forceinline__ tk_u32x4 load(const T* row, int c, int C) {
+    if (ALIGNED) return *reinterpret_cast<const tk_u32x4*>(row + c);
+    if (c + VEC <= C) return *reinterpret_cast<const tk_u32x4_at2*>(row + c);
+    tk_u32x4 q = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < VEC - 1; ++i)
+      if (c + i < C) {
+        if (sizeof(T) == 4) q[i] = __builtin_bit_cast(unsigned, tk_get(reinterpret_cast<const float*>(row) + c + i));
+        else q[i >> 1] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[c + i] << (16 * (i & 1));
+      }
+    return q;
+  }
+  static __device__ __forceinline__ void unpack(const tk_u32x4& q, float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 2) {
+      TkVec<unsigned short, 8>::unpack(q, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(q[i]);
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, int c, int C, const float (&v)[VEC]) {
+    tk_u32x4 q;
+    if constexpr (sizeof(T) == 2) q = TkVec<unsigned short, 8>::pack(v);
+    else q = __builtin_bit_cast(tk_u32x4, f32x4{v[0], v[1], v[2], v[3]});
+    if (ALIGNED) {
+      *reinterpret_cast<tk_u32x4*>(row + c) = q;
+    } else if (c + VEC <= C) {
+      *reinterpret_cast<tk_u32x4_at2*>(row + c) = q;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC - 1; ++i)
+        if (c + i < C) tk_put(row + c + i, v[i]);
+    }
+  }
+};
+
 template <typename T> struct TkVec<T, 1> {
   static __device__ __forceinline__ void load(const T* p, float (&v)[1]) { v[0] = tk_get(p); }
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { tk_put(p, v[0]); }
 };
 
-// A parameter vector (weight, bias) of either type, chosen by a wave-uniform flag.
+// VEC elements at c of a parameter vector (weight, bias) of C elements and either type (a wave-uniform flag); `rest` past
+// its end.
 template <int VEC>
-__device__ __forceinline__ void tk_load_param(const void* p, int bf16, long at, float (&v)[VEC]) {
+__device__ __forceinline__ void tk_load_param(const void* p, int bf16, int c, int C, float rest, float (&v)[VEC]) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = bf16 ? tk_bf2f(static_cast<const unsigned short*>(p)[at + i]) : static_cast<const float*>(p)[at + i];
+  for (int i = 0; i < VEC; ++i)
+    v[i] = c + i >= C ? rest : bf16 ? tk_bf2f(static_cast<const unsigned short*>(p)[c + i]) : static_cast<const float*>(p)[c + i];
 }
 
 // Every lane ends with the sum over the wave.

@@ -21,13 +21,16 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
 
 
 def same_device(what: str, first: torch.Tensor, *others) -> None:
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on different devices: {first.device} vs {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices: {dev} vs {t.device}")
 
 
 def rows_2d(t: torch.Tensor, cols: int):
-    """``t`` as rows of ``cols`` elements and the distance between them; a copy only where no such view exists."""
+    """``t`` (last axis of ``cols`` elements) as rows and the distance between them; a copy only where no such view exists."""
+    if t.is_contiguous():
+        return t, cols
     r = t.reshape(-1, cols)
     ld = r.stride(0) if r.shape[0] > 1 else cols
     if (cols > 1 and r.stride(1) != 1) or ld < cols:
@@ -37,10 +40,11 @@ def rows_2d(t: torch.Tensor, cols: int):
 
 def launch(what: str, fn, t: torch.Tensor, *args) -> None:
     """``fn(*args, stream)`` on the current stream of ``t``'s device, whatever the current device is."""
-    if t.device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
     else:
-        with torch.cuda.device(t.device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
     if rc:
         _lib.check(rc, what)

@@ -44,13 +44,21 @@ def _kernels():
 
 
 class LayerNormResult:
-    """``y``, the normalised tensor ``h`` (``x``, or ``x + residual`` as stored) and its float32 row statistics, which the
-    backward pass reads."""
+    """``y``, the normalised tensor ``h`` (``x``, or ``x + residual`` as stored) and its float32 row statistics ``stats``
+    [2, rows] = (mean, 1 / standard deviation), which the backward pass reads."""
 
-    __slots__ = ("y", "h", "mean", "rstd")
+    __slots__ = ("y", "h", "stats")
 
-    def __init__(self, y, h, mean, rstd):
-        self.y, self.h, self.mean, self.rstd = y, h, mean, rstd
+    def __init__(self, y, h, stats):
+        self.y, self.h, self.stats = y, h, stats
+
+    @property
+    def mean(self) -> torch.Tensor:
+        return self.stats[0]
+
+    @property
+    def rstd(self) -> torch.Tensor:
+        return self.stats[1]
 
 
 def _param_code(what, x, weight, bias):
@@ -80,17 +88,18 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
         raise ValueError("layer_norm: eps must not be negative")
     same_device("layer_norm", x, weight, bias, residual)
     if not x.is_cuda:
-        return LayerNormResult(*reference.layer_norm(x, weight, bias, eps, residual))
+        y, h, mean, rstd = reference.layer_norm(x, weight, bias, eps, residual)
+        return LayerNormResult(y, h, torch.stack((mean, rstd)))
     x2, ldx = rows_2d(x, cols)
     r2, ldr = rows_2d(residual, cols) if residual is not None else (None, 0)
-    rows = x2.shape[0]
+    rows = x.numel() // cols
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r2 is not None else None
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    mean = stats.data_ptr()
     launch("layer_norm_fwd", _kernels().dtf_layernorm_fwd, x, x2.data_ptr(), _lib.ptr(r2), _lib.ptr(weight), _lib.ptr(bias),
-           y.data_ptr(), _lib.ptr(h), mean.data_ptr(), rstd.data_ptr(), rows, cols, ldx, ldr, dt, wcode, eps)
-    return LayerNormResult(y, x2 if h is None else h, mean, rstd)
+           y.data_ptr(), _lib.ptr(h), mean, mean + 4 * rows, rows, cols, ldx, ldr, dt, wcode, eps)
+    return LayerNormResult(y, x2 if h is None else h, stats)
 
 
 def layer_norm_bwd(dy: torch.Tensor, fwd: LayerNormResult, weight: Optional[torch.Tensor] = None,
@@ -114,7 +123,7 @@ def layer_norm_bwd(dy: torch.Tensor, fwd: LayerNormResult, weight: Optional[torc
     h2, ldh = rows_2d(h, cols)
     dy2, lddy = rows_2d(dy, cols)
     dh2, lddh = rows_2d(dh, cols) if dh is not None else (None, 0)
-    rows = h2.shape[0]
+    rows, mean = h.numel() // cols, fwd.stats.data_ptr()
     dx = torch.empty(dy.shape, dtype=h.dtype, device=h.device)
     dw = db = part = None
     if want_wgrad:
@@ -122,7 +131,7 @@ def layer_norm_bwd(dy: torch.Tensor, fwd: LayerNormResult, weight: Optional[torc
         dw, db = grads[0], grads[1]
         part = torch.empty(lib.dtf_layernorm_bwd_ws_floats(rows, cols), dtype=torch.float32, device=h.device)
     launch("layer_norm_bwd", lib.dtf_layernorm_bwd, h, dy2.data_ptr(), h2.data_ptr(), _lib.ptr(dh2), _lib.ptr(weight),
-           fwd.mean.data_ptr(), fwd.rstd.data_ptr(), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(part), rows, cols,
+           mean, mean + 4 * rows, dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(part), rows, cols,
            lddy, ldh, lddh, dt, wcode)
     return dx, dw, db
 
@@ -131,7 +140,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps):
         r = layer_norm_fwd(x, weight, bias, eps, residual)
-        ctx.save_for_backward(r.h, r.mean, r.rstd, weight)
+        ctx.save_for_backward(r.h, r.stats, weight)
         ctx.shape, ctx.has_res, ctx.has_bias = x.shape, residual is not None, bias is not None
         ctx.bdtype = bias.dtype if bias is not None else None
         ctx.set_materialize_grads(False)
@@ -140,13 +149,13 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, mean, rstd, weight = ctx.saved_tensors
+        h, stats, weight = ctx.saved_tensors
         dw = db = None
         if dy is None:
             dx = dh                                        # only the sum itself was used
         else:
             need = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-            dx, dw, db = layer_norm_bwd(dy, LayerNormResult(None, h, mean, rstd), weight, dh, want_wgrad=need)
+            dx, dw, db = layer_norm_bwd(dy, LayerNormResult(None, h, stats), weight, dh, want_wgrad=need)
             dx = dx.view(ctx.shape)
         return (dx, dx if ctx.has_res else None, dw if weight is not None else None,
                 db.to(ctx.bdtype) if db is not None and ctx.has_bias else None, None)

@@ -70,6 +70,7 @@ def test_key_widths_of_the_sort(n, v):
 def test_very_long_rows_are_split_into_larger_chunks():
     check(70000, 9, 40, torch.float32, "cuda:0", "few")
     check(530000, 7, 8, torch.bfloat16, "cuda:0", "zipf")
+    check(1100000, 1000, 8, torch.float32, "cuda:0", "zipf")          # more than 256 blocks of the sort: scanned by a launch of its own
 
 
 @pytest.mark.parametrize("dev", devices())
