@@ -4,15 +4,17 @@
 //   backward   dtable[v] = scale sum_{i: id_i = v} dy[i]     for every row of the table, zeros where no token has it
 //
 // The gradient is a segmented sum.  Tokens are sorted by id, stably, so a row's tokens stand in the order of their
-// positions; every table row is then written exactly once, as its tokens' sum or as zeros, by the workgroup that owns it:
-// no atomics on floats (the same inputs give the same bits), no zero fill beforehand, no fp32 table in between.
-//   sort    LSD radix sort of (id, position) with digits of at most 9 bits (32 KB of counters): up to 16384 tokens in ONE workgroup and launch,
-//           else count / scan / scatter launches over blocks of 4096 tokens.
-//   parts   A frequent row summed by one workgroup would take one token after the other: the sorted list is cut into chunks,
-//           and each chunk's share of a row that crosses a chunk's border is summed by a workgroup of its own.
-//   rows    32 table rows a workgroup: searches in the sorted ids give the rows' tokens, then each row is summed in fp32 (its
-//           tokens in order, or the chunks' parts in order), scaled and rounded once.
-// Bound by memory: the table's gradient is written once (V D elements), dy is read once.
+// positions; a row with tokens is then written by one workgroup: no atomics on floats (the same inputs give the same bits)
+// and no fp32 table in between.
+//   sort    LSD radix sort of (id, position) with digits of at most 9 bits (32 KB of counters): up to 16384 tokens in ONE
+//           workgroup and launch, else count / scatter launches over blocks of 4096 tokens.  The sort keeps a few CUs busy;
+//           the other workgroups of its launches fill the table's gradient with zeros meanwhile (measured apart: 39 us of
+//           sorting 16384 tokens, 25 us of filling 50001 x 1024 bf16).
+//   chunks  The sorted list is cut into chunks of 32 tokens or more, one workgroup (or part of one) each, so that frequent
+//           rows are shared: rows inside a chunk are summed in fp32, scaled, rounded once and stored; of a row that crosses
+//           the chunk's border (at most two do) the sum is kept as a part.
+//   join    The chunk in which a crossing row starts adds the row's parts in order and stores it.
+// Bound by memory: the table's gradient is written once (V D elements) and again where a row has tokens, dy is read once.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -25,7 +27,6 @@ constexpr int kSortBlock = 1024, kSortWaves = kSortBlock / 64;
 constexpr int kKeys = 4096;                      // tokens a workgroup of the multi-launch sort
 constexpr int kMaxBits = 9;
 constexpr int kScanBlocks = 256;                 // up to here a scatter block adds up the counts by itself
-constexpr int kRows = 32;                        // table rows a workgroup of the last launch
 
 // ---------------------------------------------------------------------------------------------------------- forward
 template <typename T, int VEC>
@@ -58,6 +59,19 @@ __device__ __forceinline__ int key_of(const void* ids, int ids64, long i, long V
   return id < 0 || id >= V || id == skip ? (int)V : (int)id;
 }
 
+// Zeros for the 16-byte pieces [lo, hi) of the table's gradient, by the workgroups past the first `skip` of a launch.
+struct Fill {
+  tk_u32x4* out; long lo, hi;
+};
+__device__ __forceinline__ void fill_zero(const Fill& f, int skip) {
+  const long step = (long)(gridDim.x - skip) * kSortBlock;
+  for (long i = f.lo + (long)(blockIdx.x - skip) * kSortBlock + threadIdx.x; i < f.hi; i += step) f.out[i] = tk_u32x4{0u, 0u, 0u, 0u};
+}
+
+__global__ void emb_tail_kernel(char* out, int bytes) {
+  if ((int)threadIdx.x < bytes) out[threadIdx.x] = 0;
+}
+
 struct SortArgs {
   const void* ids; const int* key_in; const int* pos_in; int* key_out; int* pos_out; int* hist;    // hist [digits][blocks]
   long V; long long skip; int n, ids64, shift, bits, blocks, scanned;
@@ -67,12 +81,15 @@ __device__ __forceinline__ int load_key(const SortArgs& a, int i) { return a.key
 
 // Lanes of the wave whose digit equals this lane's (inactive lanes excluded): one ballot a bit.
 __device__ __forceinline__ unsigned long long same_digit(int digit, int bits, bool active) {
-  unsigned long long m = __ballot(active);
+  const unsigned long long act = __ballot(active);
+  unsigned lo = (unsigned)act, hi = (unsigned)(act >> 32);
   for (int b = 0; b < bits; ++b) {
-    const unsigned long long set = __ballot((digit >> b) & 1);
-    m &= (digit >> b) & 1 ? set : ~set;
+    const unsigned own = 0u - ((unsigned)(digit >> b) & 1u);          // all ones where this lane's bit is set
+    const unsigned long long set = __ballot(own != 0u);
+    lo &= ~((unsigned)set ^ own);
+    hi &= ~((unsigned)(set >> 32) ^ own);
   }
-  return m;
+  return ((unsigned long long)hi << 32) | lo;
 }
 
 // Exclusive prefix sum over the workgroup's threads.
@@ -111,7 +128,8 @@ __device__ __forceinline__ void rank_in_wave(const int (&key)[ROUNDS], int live,
 }
 
 // All passes in one workgroup; keys and positions stay in registers and LDS between them.
-__global__ __launch_bounds__(kSortBlock) void emb_sort_one_kernel(SortArgs a, int passes) {
+__global__ __launch_bounds__(kSortBlock) void emb_sort_one_kernel(SortArgs a, int passes, Fill f) {
+  if (blockIdx.x > 0) return fill_zero(f, 1);
   constexpr int ROUNDS = kOne / kSortBlock;
   __shared__ int s_key[kOne];
   __shared__ unsigned short s_pos[kOne];
@@ -170,7 +188,8 @@ __global__ __launch_bounds__(kSortBlock) void emb_sort_one_kernel(SortArgs a, in
   }
 }
 
-__global__ __launch_bounds__(kSortBlock) void emb_count_kernel(SortArgs a) {
+__global__ __launch_bounds__(kSortBlock) void emb_count_kernel(SortArgs a, Fill f) {
+  if ((int)blockIdx.x >= a.blocks) return fill_zero(f, a.blocks);
   __shared__ int h[1 << kMaxBits];
   const int digits = 1 << a.bits;
   const int lo = blockIdx.x * kKeys, hi = min(a.n, lo + kKeys);
@@ -203,7 +222,8 @@ __global__ __launch_bounds__(kSortBlock) void emb_scan_kernel(int* hist, int n) 
   }
 }
 
-__global__ __launch_bounds__(kSortBlock) void emb_scatter_kernel(SortArgs a) {
+__global__ __launch_bounds__(kSortBlock) void emb_scatter_kernel(SortArgs a, Fill f) {
+  if ((int)blockIdx.x >= a.blocks) return fill_zero(f, a.blocks);
   constexpr int ROUNDS = kKeys / kSortBlock;
   __shared__ int cnt[kSortWaves << kMaxBits];
   __shared__ int s_wave[kSortWaves];
@@ -255,118 +275,107 @@ __global__ __launch_bounds__(kSortBlock) void emb_scatter_kernel(SortArgs a) {
 // ------------------------------------------------------------------------------------------------------------- sums
 struct SumArgs {
   const int* key; const int* pos; const void* dy; float* part; void* out;
-  long V, lddy; int n, D, chunk, tpr_log2; float scale;
+  long V, lddy; int n, D, chunk, chunks, tpr_log2; float scale;
 };
 
+// A chunk and a column tile belong to 2^tpr_log2 threads.
 template <typename T, int VEC>
-__device__ __forceinline__ void add_tokens(const SumArgs& a, int s, int e, int c, float (&acc)[VEC]) {
-  const T* const dy = static_cast<const T*>(a.dy);
-  for (int i = s; i < e; i += 8) {
+__global__ __launch_bounds__(256) void emb_chunks_kernel(SumArgs a) {
+  const int tpr = 1 << a.tpr_log2, t = threadIdx.x & (tpr - 1);
+  const int chunk = (int)((blockIdx.x * 256u + threadIdx.x) >> a.tpr_log2), c = (blockIdx.y * tpr + t) * VEC;
+  if (chunk >= a.chunks || c >= a.D) return;
+  const int lo = chunk * a.chunk, hi = min(a.n, lo + a.chunk);
+  const T* const dy = static_cast<const T*>(a.dy) + c;
+  T* const out = static_cast<T*>(a.out) + c;
+  float* const part = a.part + (size_t)chunk * 2 * a.D + c;
+  const int first = a.key[lo];
+  bool inside = lo == 0 || a.key[lo - 1] != first;         // the current row starts in this chunk
+  float acc[VEC] = {};
+  int key[9], pos[8];
+  auto fetch = [&](int i0) {                     // keys and positions of eight tokens, and the key behind them (-1: none)
+#pragma unroll
+    for (int u = 0; u < 9; ++u) key[u] = a.key[min(i0 + u, a.n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) pos[u] = a.pos[min(i0 + u, a.n - 1)];
+  };
+  fetch(lo);
+  for (int i0 = lo; i0 < hi; i0 += 8) {
+    const int cnt = min(8, hi - i0);
+    // every load is unconditional (tokens past the end repeat the last one), so that all eight rows are under way at once
     float v[8][VEC];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (i + u < e) TkVec<T, VEC>::load(dy + a.pos[i + u] * a.lddy + c, v[u]);
+    for (int u = 0; u < 8; ++u) TkVec<T, VEC>::load(dy + pos[u] * a.lddy, v[u]);
+    int now[9];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (i + u < e) {
+    for (int u = 0; u < 9; ++u) now[u] = i0 + u < a.n ? key[u] : -1;
+    fetch(i0 + 8);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
+    for (int u = 0; u < 8; ++u) {
+      if (u >= cnt || now[u] >= a.V) continue;   // tokens without a gradient are sorted behind all others
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) acc[q] += v[u][q];
+      const bool ends = now[u + 1] != now[u];
+      if (!ends && i0 + u + 1 < hi) continue;
+      if (ends && inside) {
+        float o[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) o[q] = acc[q] * a.scale;
+        TkVec<T, VEC>::store(out + (long)now[u] * a.D, o);
+      } else {                                   // part 0: of the chunk's first row, part 1: of its last, if it is another
+        float* const p = part + (now[u] == first ? 0 : a.D);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) p[q] = acc[q];
       }
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
+      inside = true;
+    }
   }
 }
 
-// Workgroup (chunk, column tile): the chunk's share of a row whose tokens cross the chunk's border; at most two do: the row
-// of the chunk's first token (part 0) and, if it is another, the row of its last token (part 1).
+// Workgroup (chunk, 64 pieces of columns); the four waves take a quarter of the row's parts each, in order.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void emb_parts_kernel(SumArgs a) {
-  const int lo = blockIdx.x * a.chunk, hi = min(a.n, lo + a.chunk), c = (blockIdx.y * 256 + threadIdx.x) * VEC;
-  const int lane = threadIdx.x & 63;
-  const int first = a.key[lo], last = a.key[hi - 1];
-  int same_first = 0, same_last = 0;             // the keys are sorted: how many equal the first, the last
-  for (int i = lo; i < hi; i += 64) {
-    const int k = i + lane < hi ? a.key[i + lane] : -1;
-    same_first += (int)__popcll(__ballot(k == first));
-    same_last += (int)__popcll(__ballot(k == last));
+__global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a) {
+  __shared__ float s_acc[3][64][VEC];
+  const int chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (blockIdx.y * 64 + lane) * VEC;
+  const int lo = chunk * a.chunk, hi = min(a.n, lo + a.chunk);
+  const int v = a.key[hi - 1];
+  if (v >= a.V || hi == a.n || a.key[hi] != v) return;                 // the last row ends here
+  const bool whole = a.key[lo] == v;
+  if (whole && lo > 0 && a.key[lo - 1] == v) return;                   // it started before this chunk
+  int last = chunk;                              // the last chunk that begins with this row
+  while (true) {
+    const int k = last + 1 + lane;
+    const unsigned long long m = __ballot(k < a.chunks && a.key[min(k, a.chunks - 1) * a.chunk] == v);
+    last += m == ~0ull ? 64 : (int)__builtin_ctzll(~m);
+    if (m != ~0ull) break;
   }
-  if (c >= a.D) return;
-  const bool left = lo > 0 && a.key[lo - 1] == first, right = hi < a.n && a.key[hi] == last;
-  float* const part = a.part + (size_t)blockIdx.x * 2 * a.D + c;
-  if (first < a.V && (left || (right && first == last))) {
-    float acc[VEC] = {};
-    add_tokens<T, VEC>(a, lo, lo + same_first, c, acc);
+  const float* const p = a.part + (c < a.D ? c : 0);
+  const int count = last - chunk + 1, per = (count + 3) >> 2, k0 = chunk + wave * per, k1 = min(last + 1, k0 + per);
+  float acc[VEC] = {};
+  for (int k = k0; k < k1; k += 8) {
+    float v8[8][VEC];
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) part[q] = acc[q];
-  }
-  if (last < a.V && right && first != last) {
-    float acc[VEC] = {};
-    add_tokens<T, VEC>(a, hi - same_last, hi, c, acc);
+    for (int u = 0; u < 8; ++u) {                // past the end: the last part again, not added
+      const int at = min(k + u, last);
+      const float* const q8 = p + ((size_t)at * 2 + (at == chunk && !whole ? 1 : 0)) * a.D;
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) part[a.D + q] = acc[q];
-  }
-}
-
-// Workgroup (32 table rows, column tile); 2^tpr_log2 threads a row.  The rows lie gridDim.x apart: frequent tokens often have
-// neighbouring ids, and 32 frequent rows one after the other would be the launch's last workgroup (measured: 16384 tokens
-// with frequencies 1 / k on 50001 x 1024, neighbouring rows 327 us).
-template <typename T, int VEC>
-__global__ __launch_bounds__(256) void emb_rows_kernel(SumArgs a) {
-  __shared__ int s_key[257], s_at[2 * kRows];
-  const int tid = threadIdx.x;
-  // where each row's tokens start and end: a sample of 256 keys in LDS, then binary search between two of them
-  const int per = (a.n + 255) / 256;
-  s_key[tid] = per && (long)tid * per < a.n ? a.key[tid * per] : 0x7fffffff;
-  __syncthreads();
-  if (tid < 2 * kRows) {
-    const long v = (long)blockIdx.x + (long)(tid >> 1) * gridDim.x + (tid & 1);
-    int b = 0;                                   // samples below v
-    for (int half = 128; half > 0; half >>= 1)
-      if (s_key[b + half - 1] < v) b += half;
-    if (b < 256 && s_key[b] < v) ++b;
-    int lo = b > 0 ? (b - 1) * per : 0, len = b > 0 ? min(a.n - lo, per) : 0;
-    while (len > 0) {
-      const int half = len >> 1;
-      if (a.key[lo + half] < v) { lo += half + 1; len -= half + 1; } else len = half;
-    }
-    s_at[tid] = lo;
-  }
-  __syncthreads();
-  const int tpr = 1 << a.tpr_log2, t = tid & (tpr - 1);
-  const int c = (blockIdx.y * tpr + t) * VEC;
-  if (c >= a.D) return;
-  T* const out = static_cast<T*>(a.out);
-  for (int r = tid >> a.tpr_log2; r < kRows; r += 256 >> a.tpr_log2) {
-    const long v = (long)blockIdx.x + (long)r * gridDim.x;
-    if (v >= a.V) break;
-    const int s = s_at[2 * r], e = s_at[2 * r + 1];
-    float acc[VEC] = {};
-    const int k0 = s / a.chunk, k1 = (e - 1) / a.chunk;
-    if (e == s || k0 == k1) {
-      add_tokens<T, VEC>(a, s, e, c, acc);
-    } else {                                     // the row crosses a border: the chunks' parts, in order
-      const float* const p = a.part + c;
-      if (s > k0 * a.chunk) {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) acc[q] = p[((size_t)k0 * 2 + 1) * a.D + q];
-      } else {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) acc[q] = p[(size_t)k0 * 2 * a.D + q];
-      }
-      for (int k = k0 + 1; k <= k1; k += 8) {
-        float v8[8][VEC];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-#pragma unroll
-          for (int q = 0; q < VEC; ++q) v8[u][q] = k + u <= k1 ? p[(size_t)(k + u) * 2 * a.D + q] : 0.f;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-#pragma unroll
-          for (int q = 0; q < VEC; ++q) acc[q] += v8[u][q];
-      }
+      for (int q = 0; q < VEC; ++q) v8[u][q] = q8[q];
     }
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) acc[q] *= a.scale;
-    TkVec<T, VEC>::store(out + v * a.D + c, acc);
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) acc[q] += k + u < k1 ? v8[u][q] : 0.f;
   }
+  if (wave) {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) s_acc[wave - 1][lane][q] = acc[q];
+  }
+  __syncthreads();                               // every wave took the same way here
+  if (wave || c >= a.D) return;
+#pragma unroll
+  for (int q = 0; q < VEC; ++q) acc[q] = (((acc[q] + s_acc[0][lane][q]) + s_acc[1][lane][q]) + s_acc[2][lane][q]) * a.scale;
+  TkVec<T, VEC>::store(static_cast<T*>(a.out) + (long)v * a.D + c, acc);
 }
 
 // --------------------------------------------------------------------------------------------------------- host side
@@ -382,7 +391,7 @@ EmbPlan plan(int64_t n, int64_t V, int D) {
   p.passes = (total + kMaxBits - 1) / kMaxBits;
   p.bits = (total + p.passes - 1) / p.passes;
   p.blocks = (int)((n + kKeys - 1) / kKeys);
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(32, n / 1024), 1024);
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(32, n / 4096), 1024);
   p.chunks = (int)((n + p.chunk - 1) / p.chunk);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
@@ -406,12 +415,11 @@ int row_threads_log2(int D, int vec, int most) {
 }
 
 template <typename T, int VEC>
-void sums(const SumArgs& in, int chunks, hipStream_t s) {
+void sums(const SumArgs& in, hipStream_t s) {
   SumArgs a = in;
-  if (a.n > a.chunk)                             // else no row can have more tokens than a chunk
-    hipLaunchKernelGGL((emb_parts_kernel<T, VEC>), dim3(chunks, dtf_cdiv(a.D, 256 * VEC)), dim3(256), 0, s, a);
   a.tpr_log2 = row_threads_log2(a.D, VEC, 256);
-  hipLaunchKernelGGL((emb_rows_kernel<T, VEC>), dim3((unsigned)((a.V + kRows - 1) / kRows), dtf_cdiv(a.D, VEC << a.tpr_log2)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((emb_chunks_kernel<T, VEC>), dim3((unsigned)((((long)a.chunks << a.tpr_log2) + 255) / 256), dtf_cdiv(a.D, VEC << a.tpr_log2)), dim3(256), 0, s, a);
+  if (a.chunks > 1) hipLaunchKernelGGL((emb_join_kernel<T, VEC>), dim3(a.chunks - 1, dtf_cdiv(a.D, 64 * VEC)), dim3(256), 0, s, a);
 }
 }  // namespace
 
@@ -450,15 +458,22 @@ DTF_EXPORT int dtf_embedding_bwd(const void* ids, int ids64, const void* dy, voi
   if (const int rc = check(n, V, D, dtype)) return rc;
   if (lddy < D) return DTF_ERR_SHAPE;
   if (!out || (n > 0 && (!ids || !dy || !ws))) return DTF_ERR_ARG;
+  if (!dtf_aligned16(out)) return DTF_ERR_ALIGN;
   const EmbPlan p = plan(n, V, D);
   if (n > 0 && ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   char* const w = static_cast<char*>(ws);
   int* const key_a = reinterpret_cast<int*>(w + p.key_a), * const pos_a = reinterpret_cast<int*>(w + p.pos_a);
   int* const key_b = reinterpret_cast<int*>(w + p.key_b), * const pos_b = reinterpret_cast<int*>(w + p.pos_b);
   SortArgs a = {ids, nullptr, nullptr, key_a, pos_a, reinterpret_cast<int*>(w + p.hist), (long)V, skip, (int)n, ids64, 0, p.bits, p.blocks, p.blocks > kScanBlocks};
-  if (n > 0 && n <= kOne) {
-    hipLaunchKernelGGL(emb_sort_one_kernel, dim3(1), dim3(kSortBlock), 0, s, a, p.passes);
-  } else if (n > 0) {
+  // zeros, in equal shares of the sort's launches; the bytes behind the last whole 16-byte piece by themselves
+  const int64_t bytes = V * D * (dtype == TK_BF16 ? 2 : 4), pieces = bytes / 16;
+  const int shares = n <= kOne ? 1 : 2 * p.passes;
+  auto fill = [&](int share) { return Fill{static_cast<tk_u32x4*>(out), (long)(pieces * share / shares), (long)(pieces * (share + 1) / shares)}; };
+  const unsigned fillers = (unsigned)std::min<int64_t>(511, (pieces / shares + kSortBlock - 1) / kSortBlock);
+  if (bytes % 16) hipLaunchKernelGGL(emb_tail_kernel, dim3(1), dim3(64), 0, s, static_cast<char*>(out) + pieces * 16, (int)(bytes % 16));
+  if (n <= kOne) {
+    hipLaunchKernelGGL(emb_sort_one_kernel, dim3(1 + fillers), dim3(kSortBlock), 0, s, a, n > 0 ? p.passes : 0, fill(0));
+  } else {
     for (int k = 0; k < p.passes; ++k) {
       const bool to_a = ((p.passes - 1 - k) & 1) == 0;       // the last pass ends in a
       a.key_in = k == 0 ? nullptr : to_a ? key_b : key_a;
@@ -466,15 +481,17 @@ DTF_EXPORT int dtf_embedding_bwd(const void* ids, int ids64, const void* dy, voi
       a.key_out = to_a ? key_a : key_b;
       a.pos_out = to_a ? pos_a : pos_b;
       a.shift = k * p.bits;
-      hipLaunchKernelGGL(emb_count_kernel, dim3(p.blocks), dim3(kSortBlock), 0, s, a);
+      hipLaunchKernelGGL(emb_count_kernel, dim3(p.blocks + fillers), dim3(kSortBlock), 0, s, a, fill(2 * k));
       if (a.scanned) hipLaunchKernelGGL(emb_scan_kernel, dim3(1), dim3(kSortBlock), 0, s, a.hist, p.blocks << p.bits);
-      hipLaunchKernelGGL(emb_scatter_kernel, dim3(p.blocks), dim3(kSortBlock), 0, s, a);
+      hipLaunchKernelGGL(emb_scatter_kernel, dim3(p.blocks + fillers), dim3(kSortBlock), 0, s, a, fill(2 * k + 1));
     }
   }
-  const SumArgs q = {key_a, pos_a, dy, reinterpret_cast<float*>(w + p.part), out, (long)V, (long)lddy, (int)n, D, p.chunk, 0, scale};
-  const int vec = dtype == TK_BF16 ? 8 : 4;
-  const bool v = D % vec == 0 && lddy % vec == 0 && dtf_aligned16(dy) && dtf_aligned16(out);
-  if (dtype == TK_BF16) v ? sums<unsigned short, 8>(q, p.chunks, s) : sums<unsigned short, 1>(q, p.chunks, s);
-  else v ? sums<float, 4>(q, p.chunks, s) : sums<float, 1>(q, p.chunks, s);
+  if (n > 0) {
+    const SumArgs q = {key_a, pos_a, dy, reinterpret_cast<float*>(w + p.part), out, (long)V, (long)lddy, (int)n, D, p.chunk, p.chunks, 0, scale};
+    const int vec = dtype == TK_BF16 ? 8 : 4;
+    const bool v = D % vec == 0 && lddy % vec == 0 && dtf_aligned16(dy);
+    if (dtype == TK_BF16) v ? sums<unsigned short, 8>(q, s) : sums<unsigned short, 1>(q, s);
+    else v ? sums<float, 4>(q, s) : sums<float, 1>(q, s);
+  }
   return dtf_check_launch();
 }

@@ -101,6 +101,15 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LnArgs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) P::unpack(raw[j], v[j]);
   }
+  float w[NV][VEC], b[NV][VEC];                // asked for before the sums, needed after them
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * TPR + t) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { w[j][i] = 1.f; b[j][i] = 0.f; }
+    if (a.w && c < a.C) tk_load_param<VEC>(a.w, a.w_bf16, c, AL ? 0x7fffffff : a.C, 1.f, w[j]);
+    if (a.b && c < a.C) tk_load_param<VEC>(a.b, a.w_bf16, c, AL ? 0x7fffffff : a.C, 0.f, b[j]);
+  }
   int half = 0;
   float s[1] = {0.f};
 #pragma unroll
@@ -132,13 +141,9 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LnArgs a) {
   for (int j = 0; j < NV; ++j) {
     const int c = (j * TPR + t) * VEC;
     if (c < a.C) {
-      float w[VEC], b[VEC], o[VEC];
+      float o[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) { w[i] = 1.f; b[i] = 0.f; }
-      if (a.w) tk_load_param<VEC>(a.w, a.w_bf16, c, AL ? 0x7fffffff : a.C, 1.f, w);
-      if (a.b) tk_load_param<VEC>(a.b, a.w_bf16, c, AL ? 0x7fffffff : a.C, 0.f, b);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i] = fmaf(v[j][i] * rstd, w[i], b[i]);
+      for (int i = 0; i < VEC; ++i) o[i] = fmaf(v[j][i] * rstd, w[j][i], b[j][i]);
       P::store(y, c, a.C, o);
     }
   }

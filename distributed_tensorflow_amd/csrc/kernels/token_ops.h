@@ -92,13 +92,35 @@ template <typename T> struct TkVec<T, 1> {
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { tk_put(p, v[0]); }
 };
 
-// VEC elements at c of a parameter vector (weight, bias) of C elements and either type (a wave-uniform flag); `rest` past
-// its end.
+// VEC elements at c of a parameter vector (weight, bias) of C elements and either type (a wave-uniform flag), by 16-byte
+// accesses at the elements' own alignment; `rest` past its end.
+typedef f32x4 tk_f32x4_at4 __attribute__((aligned(4)));
 template <int VEC>
 __device__ __forceinline__ void tk_load_param(const void* p, int bf16, int c, int C, float rest, float (&v)[VEC]) {
+  if (VEC >= 4 && c + VEC <= C) {
+    if (bf16) {
+      const unsigned short* const q = static_cast<const unsigned short*>(p) + c;
+      if constexpr (VEC == 8) {
+        TkVec<unsigned short, 8>::unpack(*reinterpret_cast<const tk_u32x4_at2*>(q), v);
+      } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    v[i] = c + i >= C ? rest : bf16 ? tk_bf2f(static_cast<const unsigned short*>(p)[c + i]) : static_cast<const float*>(p)[c + i];
+        for (int i = 0; i < VEC; ++i) v[i] = tk_bf2f(q[i]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC / 4; ++k) {
+        const f32x4 q = *reinterpret_cast<const tk_f32x4_at4*>(static_cast<const float*>(p) + c + 4 * k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * k + i] = q[i];
+      }
+    }
+  } else if (bf16) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = c + i < C ? tk_bf2f(static_cast<const unsigned short*>(p)[c + i]) : rest;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = c + i < C ? static_cast<const float*>(p)[c + i] : rest;
+  }
 }
 
 // Every lane ends with the sum over the wave.

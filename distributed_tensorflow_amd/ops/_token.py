@@ -42,9 +42,9 @@ def launch(what: str, fn, t: torch.Tensor, *args) -> None:
     """``fn(*args, stream)`` on the current stream of ``t``'s device, whatever the current device is."""
     index = t.device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)

@@ -65,7 +65,7 @@ def dropout_apply(x: torch.Tensor, rate: float, seed: int, step: Union[int, torc
         return reference.dropout(x, rate, seed, value, residual)
     xc = x.contiguous()
     rc = residual.contiguous() if residual is not None else None
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     launch("dropout", _kernels().dtf_dropout, x, xc.data_ptr(), _lib.ptr(rc), y.data_ptr(), xc.numel(), dt, rate, seed,
            0 if step_t is not None else step, _lib.ptr(step_t), _lib.ptr(used))
     return y

@@ -65,7 +65,7 @@ def embedding_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
         return reference.embedding(ids, table, scale)
     t2, ldt = rows_2d(table, table.shape[1])
     ids = ids.contiguous()
-    y = torch.empty((*ids.shape, table.shape[1]), dtype=table.dtype, device=table.device)
+    y = table.new_empty((*ids.shape, table.shape[1]))
     launch("embedding_fwd", _kernels().dtf_embedding_fwd, table, ids.data_ptr(), int(ids.dtype == torch.int64), t2.data_ptr(), y.data_ptr(),
            ids.numel(), table.shape[0], table.shape[1], ldt, dt, scale)
     return y

@@ -93,9 +93,9 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     x2, ldx = rows_2d(x, cols)
     r2, ldr = rows_2d(residual, cols) if residual is not None else (None, 0)
     rows = x.numel() // cols
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r2 is not None else None
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    y = x.new_empty(x.shape)
+    h = x.new_empty(x.shape) if r2 is not None else None
+    stats = x.new_empty((2, rows), dtype=torch.float32)
     mean = stats.data_ptr()
     launch("layer_norm_fwd", _kernels().dtf_layernorm_fwd, x, x2.data_ptr(), _lib.ptr(r2), _lib.ptr(weight), _lib.ptr(bias),
            y.data_ptr(), _lib.ptr(h), mean, mean + 4 * rows, rows, cols, ldx, ldr, dt, wcode, eps)
@@ -124,12 +124,12 @@ def layer_norm_bwd(dy: torch.Tensor, fwd: LayerNormResult, weight: Optional[torc
     dy2, lddy = rows_2d(dy, cols)
     dh2, lddh = rows_2d(dh, cols) if dh is not None else (None, 0)
     rows, mean = h.numel() // cols, fwd.stats.data_ptr()
-    dx = torch.empty(dy.shape, dtype=h.dtype, device=h.device)
+    dx = h.new_empty(dy.shape)
     dw = db = part = None
     if want_wgrad:
-        grads = torch.empty((2, cols), dtype=wdtype, device=h.device)
+        grads = h.new_empty((2, cols), dtype=wdtype)
         dw, db = grads[0], grads[1]
-        part = torch.empty(lib.dtf_layernorm_bwd_ws_floats(rows, cols), dtype=torch.float32, device=h.device)
+        part = h.new_empty(lib.dtf_layernorm_bwd_ws_floats(rows, cols), dtype=torch.float32)
     launch("layer_norm_bwd", lib.dtf_layernorm_bwd, h, dy2.data_ptr(), h2.data_ptr(), _lib.ptr(dh2), _lib.ptr(weight),
            mean, mean + 4 * rows, dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(part), rows, cols,
            lddy, ldh, lddh, dt, wcode)
