@@ -18,7 +18,7 @@
 // type (bf16: half a step 2^-8 of each element, the same rounding that any bf16 product of dz has).
 //
 // Kernels: the 8-wave 256x256 GEMM (gemm_pingpong.h) for bf16 where its blocks fill the chip, the 4-wave 128x128 one
-// (gemm_tiled.h) otherwise and for fp32.  Widths that are no multiple of 16 bytes, unaligned or strided operands go through
+// (gemm_tiled.h) otherwise and for fp32; logits of few rows or columns by a kernel that shares K between the waves.  Widths that are no multiple of 16 bytes, unaligned or strided operands go through
 // zero-padded copies, piece by piece.
 #include <hip/hip_runtime.h>
 
@@ -282,6 +282,56 @@ struct VxGemm : DtfGemmArgs {
   }
 };
 
+// Few rows, or few columns: 16 rows x 64 columns a workgroup, the four waves share K (64 bytes of a row a step, wave by
+// wave), operands straight from memory into the matrix instructions: one wave's 20 loads in flight, no staging, no barrier
+// in the loop.  Every row of W is read by ceil(M / 16) workgroups, next to each other on one XCD.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
+  constexpr int PER16 = Elem<T>::PER16, AHEAD = 4;
+  __shared__ float s_acc[3][16][64];
+  __shared__ __attribute__((aligned(16))) unsigned char s_out[2048];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
+  const int tiles_m = (p.M + 15) >> 4, wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
+  const int m0 = (wg % tiles_m) * 16, n0 = (wg / tiles_m) * 64;
+  const rsrc_t ra = make_rsrc(p.A, p.a_bytes), rb = make_rsrc(p.B, p.b_bytes);
+  const unsigned a_off = m0 + fr < p.M ? (unsigned)(m0 + fr) * (unsigned)p.lda * (unsigned)sizeof(T) : kOOB;
+  unsigned b_off[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b_off[j] = n0 + 16 * j + fr < p.N ? (unsigned)(n0 + 16 * j + fr) * (unsigned)p.ldb * (unsigned)sizeof(T) : kOOB;
+  f32x4 acc[1][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (p.K + 4 * PER16 - 1) / (4 * PER16);
+  for (int s = wave; s < steps; s += 4 * AHEAD) {
+    u32x4 a[AHEAD], b[AHEAD][4];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = (s + 4 * u) * 4 + g;           // 16-byte piece of the row
+      const bool in = k * PER16 < p.K;
+      a[u] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(in && a_off != kOOB ? a_off + k * 16u : kOOB), 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(in && b_off[j] != kOOB ? b_off[j] + k * 16u : kOOB), 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma_slot<T>(a[u], b[u][j], acc[0][j]);
+  }
+  if (wave) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_acc[wave - 1][4 * j + r][lane] = acc[0][j][r];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[0][j][r] = ((acc[0][j][r] + s_acc[0][4 * j + r][lane]) + s_acc[1][4 * j + r][lane]) + s_acc[2][4 * j + r][lane];
+  p.template epilogue<EPI>(acc, s_out, m0, n0, lane);
+}
+
 // ------------------------------------------------------------------------------------------------- streaming helpers
 // dst[r, 0 .. ldd) = src[r, 0 .. cols) and zeros: an aligned, padded copy in the operands' type.
 template <typename TS, typename TD>
@@ -474,6 +524,12 @@ bool use_pp(int dtype, long m, long n, long k, int splits) {
   return dtype == TK_BF16 && m >= 256 && n >= 256 && k / splits >= 256 && ((m + 255) / 256) * ((n + 255) / 256) * splits >= 192;
 }
 
+// 128x128 blocks would leave most CUs idle, or their rows mostly empty
+bool use_skinny(long m, long n) { return m <= 16 || ((m + 127) / 128) * ((n + 127) / 128) < 128; }
+
+// Rows of a wave's block in the logits' epilogue
+int wave_rows(const VxGemm& a) { return use_skinny(a.M, a.N) ? 16 : use_pp(a.dtype, a.M, a.N, a.K, 1) ? 128 : 64; }
+
 template <int EPI>
 void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
   if (use_pp(a.dtype, a.M, a.N, a.K, splits)) {
@@ -484,6 +540,14 @@ void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
     if (a.dtype == TK_BF16) hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, EPI, 4, 4, VxGemm>), g, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((gemm_tiled_kernel<unsigned int, EPI, 4, 4, VxGemm>), g, dim3(256), 0, s, a);
   }
+}
+
+template <int EPI>
+void launch_logits(const VxGemm& a, hipStream_t s) {
+  if (!use_skinny(a.M, a.N)) return launch_gemm<EPI>(a, 1, s);
+  const dim3 g((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64)));
+  if (a.dtype == TK_BF16) hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI>), g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI>), g, dim3(256), 0, s, a);
 }
 
 VxGemm operands(const void* A, const void* B, int dtype, int M, int N, int K, long lda, long ldb) {
@@ -563,7 +627,7 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
     p.direct_dw = p.sw == 1 && p.Dp == a.D && dtf_aligned16(a.dW);
     if (!p.direct_dx || (a.dtype == TK_BF16 && p.pieces > 1)) p.dx32 = take(at, (size_t)p.sx * a.N * p.Dp * 4);
     if (!p.direct_dw) p.dw32 = take(at, (size_t)p.sw * p.Vp * p.Dp * 4);
-    if (a.dbias) p.db = take(at, (size_t)((a.N + 63) / 64 + 4) * p.Vp * 4);
+    if (a.dbias) p.db = take(at, (size_t)(a.N / 16 + 4) * p.Vp * 4);       // one row of partial sums for every 16 rows at most
   }
   p.total = at;
   return p;
@@ -645,7 +709,7 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.part = reinterpret_cast<float2*>(ws + p.part);
     g.target = reinterpret_cast<float2*>(ws + p.target);
     g.v0 = (int)v0;
-    launch_gemm<VX_LSE>(g, 1, s);
+    launch_logits<VX_LSE>(g, s);
   }
   VxJoin j = {reinterpret_cast<const float2*>(ws + p.part), reinterpret_cast<const float2*>(ws + p.target), a.labels, a.lse, a.loss_rows, a.loss,
               a.counts, reinterpret_cast<float*>(ws + p.blk), reinterpret_cast<int*>(ws + p.blk + p.blocks * 4), a.N, (int)p.strips, (int)p.blocks,
@@ -695,10 +759,9 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.Ct = ws + p.dzt;
     g.ldct = (int)p.Np;
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
-    launch_gemm<VX_DZ>(g, 1, s);
+    launch_logits<VX_DZ>(g, s);
     if (a.dbias) {
-      const int wave_rows = use_pp(g.dtype, g.M, g.N, g.K, 1) ? 128 : 64;
-      hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows), (int)n, a.dbias + v0, scale);
+      hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g)), (int)n, a.dbias + v0, scale);
     }
     if (a.dX) {
       transpose(W, ws + p.wt, n, p.Dp, ldw, np, a.dtype, s);
