@@ -60,7 +60,8 @@ __device__ __forceinline__ float pp_bf2f(unsigned short h) { return __uint_as_fl
 
 template <int EPI, class Args>
 __global__ __launch_bounds__(512) void gemm_pp_kernel(Args p) {
-  if constexpr (EPI >= EPI_CUSTOM) p.select(blockIdx.y);
+  int own_wg = 0;
+  if constexpr (EPI >= EPI_CUSTOM) own_wg = p.select();
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * 4 * 16384];   // [buffer][A0 A1 B0 B1][128 rows x 128 B]
 
   const int tid = threadIdx.x;
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(512) void gemm_pp_kernel(Args p) {
   const int kper = (EPI == EPI_WGRAD && p.ksplit > 1) ? (((p.K + p.ksplit - 1) / p.ksplit + 127) & ~127) : p.K;
   const int k_begin = split * kper;
   const int k_len = min(p.K - k_begin, kper);          // <= 0 for a split past the end: every load is out of range
-  const int wg = dtf_xcd_remap((int)blockIdx.x - split * ntile, ntile);
+  const int wg = EPI >= EPI_CUSTOM ? own_wg : dtf_xcd_remap((int)blockIdx.x - split * ntile, ntile);
   // consecutive (remapped) ids walk down a band of 8 row-tiles: the A panels and one B panel stay in that XCD's L2
   const int band = 8;
   const int per_band = band * tiles_n;
@@ -105,14 +106,20 @@ __global__ __launch_bounds__(512) void gemm_pp_kernel(Args p) {
   const unsigned a_half = 64u * (unsigned)p.lda * 2u, b_half = 32u * (unsigned)p.ldb * 2u;
   // K-tiles: an even number that covers K; 16-byte chunks at or past K are requested out of range (the range check
   // of the buffer load then delivers zeros), so K only has to be a multiple of 8
-  const int nk = ((max(k_len, 0) + 127) >> 7) << 1;
+  const int nk_plane = ((max(k_len, 0) + 127) >> 7) << 1;
+  const int nk = EPI >= EPI_PLANES ? 6 * nk_plane : nk_plane;
   const int klim = k_len * 2 - (int)kchunk;          // a lane's chunk of K-tile kt is inside its K range iff kt*128 < klim
   lds_byte_t* const lds3 = (lds_byte_t*)(lds) + wave * 1024;
 
   auto stage = [&](int buf, int region, int kt) {
-    const bool live = kt * 128 < klim;               // also false for every K-tile past the last
+    bool live = kt * 128 < klim;                     // also false for every K-tile past the last
     const unsigned half = (unsigned)(region & 1);
-    const unsigned so = (unsigned)kt * 128u + half * (region < REG_B0 ? a_half : b_half);
+    unsigned so = (unsigned)kt * 128u + half * (region < REG_B0 ? a_half : b_half);
+    if constexpr (EPI >= EPI_PLANES) {
+      const GemmPlaneTile t = gemm_plane_pair(kt, nk_plane, p.a_plane, p.b_plane);
+      live = t.pair < 6 && t.tile * 128 < klim;
+      so = (unsigned)t.tile * 128u + half * (region < REG_B0 ? a_half : b_half) + (region < REG_B0 ? t.a_off : t.b_off);
+    }
     lds_byte_t* dst = lds3 + buf * 65536 + region * 16384;
     if (region < REG_B0) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, (int)(live ? a_vo[0] : kOOB), (int)so, 0, 0);
@@ -219,7 +226,7 @@ __global__ __launch_bounds__(512) void gemm_pp_kernel(Args p) {
   const int crow = m0 + wr * 128, ccol = n0 + wc * 64;          // origin of this wave's block
   if constexpr (EPI >= EPI_CUSTOM) {
     // the same accumulators as acc[row block of 16][column block of 16]
-    p.template epilogue<EPI>(reinterpret_cast<f32x4(&)[8][4]>(acc), wl, crow, ccol, lane);
+    p.template epilogue<EPI & ~EPI_PLANES, (EPI >= EPI_PLANES)>(reinterpret_cast<f32x4(&)[8][4]>(acc), wl, crow, ccol, lane);
     return;
   }
   if (EPI == EPI_WGRAD || EPI == EPI_WGRAD_OPT) {

@@ -60,7 +60,6 @@ __device__ __forceinline__ void mma_slot<unsigned int>(const u32x4& a, const u32
 //          traffic per flop.  Used for bf16 when the problem fills the chip with such blocks.
 template <typename T, int EPI, int TI, int TJ, class Args>
 __global__ __launch_bounds__(256) void gemm_tiled_kernel(Args p) {
-  if constexpr (EPI >= EPI_CUSTOM) p.select(blockIdx.y);
   constexpr int PER16 = Elem<T>::PER16;
   constexpr int BKE = 8 * PER16;             // elements per 128-byte LDS row
   constexpr int BM = 32 * TI, BN = 32 * TJ;
@@ -74,7 +73,9 @@ __global__ __launch_bounds__(256) void gemm_tiled_kernel(Args p) {
   const int wm = wave >> 1, wn = wave & 1;
 
   const int tiles_n = (p.N + BN - 1) / BN, tiles_m = (p.M + BM - 1) / BM;
-  const int wg = dtf_xcd_remap(blockIdx.x, tiles_m * tiles_n);
+  int wg;
+  if constexpr (EPI >= EPI_CUSTOM) wg = p.select();
+  else wg = dtf_xcd_remap(blockIdx.x, tiles_m * tiles_n);
   // consecutive (remapped) ids walk down a column band of 8 row-tiles: A panels and one B panel stay in L2
   const int band = 8;
   const int per_band = band * tiles_n;
@@ -103,16 +104,25 @@ __global__ __launch_bounds__(256) void gemm_tiled_kernel(Args p) {
     b_goff[c] = (n0 + row < p.N) ? (unsigned)(n0 + row) * (unsigned)p.ldb * (unsigned)sizeof(T) + (unsigned)slot * 16u : kOOB;
     lb_off[c] = (unsigned)row * 128u + (unsigned)((slot ^ (row & 7)) << 4);
   }
-  const int nstage = (p.K + BKE - 1) / BKE;
+  const int nstage_plane = (p.K + BKE - 1) / BKE;
+  const int nstage = EPI >= EPI_PLANES ? 6 * nstage_plane : nstage_plane;
   const int my_slot = tid & 7;               // (tid + 256 c) & 7 for every c
   u32x4 ra_reg[TI], rb_reg[TJ];
   auto stage_load = [&](int t) {
-    const int k0 = t * BKE;
+    int k0 = t * BKE;
+    unsigned ka = 0, kb = 0;
+    if constexpr (EPI >= EPI_PLANES) {
+      const GemmPlaneTile q = gemm_plane_pair(t, nstage_plane, p.a_plane, p.b_plane);
+      k0 = q.tile * BKE;
+      ka = q.a_off;
+      kb = q.b_off;
+    }
     const bool kin = k0 + my_slot * PER16 < p.K;           // K is a multiple of PER16 (checked by the launcher)
-    const unsigned kb = (unsigned)k0 * (unsigned)sizeof(T);
+    ka += (unsigned)k0 * (unsigned)sizeof(T);
+    kb += (unsigned)k0 * (unsigned)sizeof(T);
 #pragma unroll
     for (int c = 0; c < TI; ++c)
-      ra_reg[c] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)((kin && a_goff[c] != kOOB) ? a_goff[c] + kb : kOOB), 0, 0);
+      ra_reg[c] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)((kin && a_goff[c] != kOOB) ? a_goff[c] + ka : kOOB), 0, 0);
 #pragma unroll
     for (int c = 0; c < TJ; ++c)
       rb_reg[c] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)((kin && b_goff[c] != kOOB) ? b_goff[c] + kb : kOOB), 0, 0);
@@ -208,7 +218,7 @@ __global__ __launch_bounds__(256) void gemm_tiled_kernel(Args p) {
   if constexpr (EPI >= EPI_CUSTOM) {       // the barrier that ends the main loop leaves the staging buffers free
     static_assert(TI == 4 && TJ == 4, "one 16 KB piece of the staging buffers for each wave's 64x64 block");
     unsigned char* const wl = (wave < 2 ? lds_a[wave] : lds_b[wave - 2]);
-    p.template epilogue<EPI>(acc, wl, m0 + wm * 64, n0 + wn * 64, lane);
+    p.template epilogue<EPI & ~EPI_PLANES, (EPI >= EPI_PLANES)>(acc, wl, m0 + wm * 64, n0 + wn * 64, lane);
     return;
   }
   // ---------------- epilogue: acc[i][j][r] = C[m0 + wm*16*TI + 16i + 4g + r][n0 + wn*16*TJ + 16j + fr]

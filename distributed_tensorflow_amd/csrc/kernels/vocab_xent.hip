@@ -17,9 +17,14 @@
 // Bound by the matrix cores.  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
 // type (bf16: half a step 2^-8 of each element, the same rounding that any bf16 product of dz has).
 //
-// Kernels: the 8-wave 256x256 GEMM (gemm_pingpong.h) for bf16 where its blocks fill the chip, the 4-wave 128x128 one
-// (gemm_tiled.h) otherwise and for fp32; logits of few rows or columns by a kernel that shares K between the waves.  Widths that are no multiple of 16 bytes, unaligned or strided operands go through
-// zero-padded copies, piece by piece.
+// fp32 operands are cut into three bf16 planes, x = x0 + x1 + x2 up to 2^-26 |x| (each plane takes eight more bits), and a
+// product is the sum of the six plane products x0 w0, x0 w1, x1 w0, x0 w2, x2 w0, x1 w1, accumulated in fp32; what is left out
+// is below 2^-25 of |x w|, under an fp32 rounding.  Six bf16 matrix products cost less than one in fp32, whose matrix rate is
+// a sixteenth.  (Elements below 2^-110 lose their last planes: 10^-33 beside sums of order one.)
+//
+// Kernels: the 8-wave 256x256 GEMM (gemm_pingpong.h) where its blocks fill the chip, the 4-wave 128x128 one (gemm_tiled.h)
+// otherwise; logits of few rows or columns by a kernel that shares K between the waves (fp32: fp32 matrix instructions).
+// bf16 widths that are no multiple of 16 bytes, unaligned or strided operands go through zero-padded copies, piece by piece.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -67,18 +72,25 @@ struct VxGemm : DtfGemmArgs {
   float2* part;                                  // [strips][M]
   float2* target;                                // [M]: the label's logit, whether an earlier column of its strip reaches it
   int v0;                                        // vocabulary index of column 0
-  // VX_DZ (C = dz [M, ldc], Ct = dz^T [N, ldct]; both leading dimensions are the padded widths, padding is zeroed)
+  // VX_DZ (C = dz [M, ldc], Ct = dz^T [N, ldct]; both leading dimensions are the padded widths, padding is zeroed; of fp32
+  // operands only C, in fp32)
   const VxRow* rows;                             // padded to the block height
+  unsigned a_plane, b_plane;                     // bytes between the planes of the operands (EPI_PLANES)
   float* db_part;                                // [wave rows][N], optional
   // VX_SUM: fp32 result C32 [splits][M, ldc32] (accumulate: added to what is there), times *scale if given; with C the
   // sum goes there as bf16 [M, ldc] instead
   const float* scale;
   int kper, accumulate;
 
-  __device__ __forceinline__ void select(int y) {
+  // The block's K range (split blockIdx.y of a grid of tiles x splits) and tile.  Workgroups go to the 8 XCDs in turn; the
+  // remap over the whole grid puts the tiles of one K range next to each other on one XCD, where they share its panels.
+  __device__ __forceinline__ int select() {
+    const int tiles = (int)gridDim.x;
+    const int lin = dtf_xcd_remap((int)(blockIdx.y * gridDim.x + blockIdx.x), tiles * (int)gridDim.y);
+    const int y = lin / tiles;
     if (kper > 0) {
       const int k0 = y * kper;
-      const unsigned off = (unsigned)k0 * (dtype == 1 ? 2u : 4u);
+      const unsigned off = (unsigned)k0 * 2u;
       A = static_cast<const char*>(A) + off;
       B = static_cast<const char*>(B) + off;
       a_bytes -= off;
@@ -86,10 +98,11 @@ struct VxGemm : DtfGemmArgs {
       K = min(kper, K - k0);
       C32 += (size_t)y * M * ldc32;
     }
+    return lin - y * tiles;
   }
 
   // acc[ri][cj][r] = C[crow + 16 ri + 4 (lane >> 4) + r][ccol + 16 cj + (lane & 15)]; wl: 16 KB of LDS of this wave
-  template <int EPI, int RI>
+  template <int EPI, bool F32, int RI>
   __device__ __forceinline__ void epilogue(f32x4 (&acc)[RI][4], unsigned char* wl, int crow, int ccol, int lane) const {
     if (ccol >= N) return;                       // wave-uniform: no column of this block exists
     const int fr = lane & 15, g = lane >> 4;
@@ -172,32 +185,26 @@ struct VxGemm : DtfGemmArgs {
           if (g == 0 && col < N) db_part[(size_t)(crow / (16 * RI)) * N + col] = v;
         }
       }
-      if (dtype == 1) store_dz16<RI>(acc, wl, crow, ccol, lane);
-      else store_dz32<RI>(acc, crow, ccol, lane);
+      if constexpr (F32) {
+        float* const c = static_cast<float*>(C);
+#pragma unroll
+        for (int ri = 0; ri < RI; ++ri)
+#pragma unroll
+          for (int cj = 0; cj < 4; ++cj)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = crow + 16 * ri + 4 * g + r, col = ccol + 16 * cj + fr;
+              if (row < M && col < ldc) c[(size_t)row * ldc + col] = acc[ri][cj][r];
+            }
+      } else {
+        store_dz<RI>(acc, wl, crow, ccol, lane);
+      }
     }
   }
 
-  // fp32: straight from the result layout (a lane holds four rows of a column)
+  // Both images are turned in LDS, so that every global store is 16 bytes a lane.
   template <int RI>
-  __device__ __forceinline__ void store_dz32(const f32x4 (&acc)[RI][4], int crow, int ccol, int lane) const {
-    const int fr = lane & 15, g = lane >> 4;
-    float* const c = static_cast<float*>(C);
-    float* const ct = static_cast<float*>(Ct);
-#pragma unroll
-    for (int ri = 0; ri < RI; ++ri)
-#pragma unroll
-      for (int cj = 0; cj < 4; ++cj) {
-        const int row = crow + 16 * ri + 4 * g, col = ccol + 16 * cj + fr;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (row + r < M && col < ldc) c[(size_t)(row + r) * ldc + col] = acc[ri][cj][r];
-        if (col < N && row < ldct) *reinterpret_cast<f32x4*>(&ct[(size_t)col * ldct + row]) = acc[ri][cj];   // ldct is a multiple of 4
-      }
-  }
-
-  // bf16: both images are turned in LDS, so that every global store is 16 bytes a lane
-  template <int RI>
-  __device__ __forceinline__ void store_dz16(const f32x4 (&acc)[RI][4], unsigned char* wl, int crow, int ccol, int lane) const {
+  __device__ __forceinline__ void store_dz(const f32x4 (&acc)[RI][4], unsigned char* wl, int crow, int ccol, int lane) const {
     constexpr int CH = 2 * RI;                   // 16-byte chunks of a transposed row (16 RI rows of dz)
     const int fr = lane & 15, g = lane >> 4;
     unsigned short* const c = static_cast<unsigned short*>(C);
@@ -329,7 +336,7 @@ __global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[0][j][r] = ((acc[0][j][r] + s_acc[0][4 * j + r][lane]) + s_acc[1][4 * j + r][lane]) + s_acc[2][4 * j + r][lane];
-  p.template epilogue<EPI>(acc, s_out, m0, n0, lane);
+  p.template epilogue<EPI, sizeof(T) == 4>(acc, s_out, m0, n0, lane);
 }
 
 // ------------------------------------------------------------------------------------------------- streaming helpers
@@ -343,28 +350,69 @@ __global__ __launch_bounds__(256) void vx_pack_kernel(const TS* __restrict__ src
 }
 
 // dst[c, r] = src[r, c] for r < M, c < N; zeros for r in [M, ldt).  64 x 64 tiles through LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void vx_transpose_kernel(const T* __restrict__ src, T* __restrict__ dst, int M, int N, long lds_, int ldt) {
-  constexpr int PER16 = 16 / sizeof(T);
-  __shared__ T tile[64][64 + PER16];
+__global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short* __restrict__ src, unsigned short* __restrict__ dst, int M, int N, long lds_, int ldt) {
+  __shared__ unsigned short tile[64][72];
   const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-  constexpr int CH = 64 / PER16;               // 16-byte chunks of a tile row
 #pragma unroll
-  for (int i = 0; i < CH / 4; ++i) {
-    const int id = threadIdx.x + 256 * i, rr = id / CH, ch = id % CH;
+  for (int i = 0; i < 2; ++i) {
+    const int id = threadIdx.x + 256 * i, rr = id >> 3, ch = id & 7;
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (r0 + rr < M && c0 + ch * PER16 < N) v = *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + rr) * lds_ + c0 + ch * PER16);
-    *reinterpret_cast<u32x4*>(&tile[rr][ch * PER16]) = v;
+    if (r0 + rr < M && c0 + ch * 8 < N) v = *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + rr) * lds_ + c0 + ch * 8);
+    *reinterpret_cast<u32x4*>(&tile[rr][ch * 8]) = v;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < CH / 4; ++i) {
-    const int id = threadIdx.x + 256 * i, cc = id / CH, ch = id % CH;
-    if (c0 + cc >= N || r0 + ch * PER16 >= ldt) continue;
-    alignas(16) T e[PER16];
+  for (int i = 0; i < 2; ++i) {
+    const int id = threadIdx.x + 256 * i, cc = id >> 3, ch = id & 7;
+    if (c0 + cc >= N || r0 + ch * 8 >= ldt) continue;
+    unsigned e[4];
 #pragma unroll
-    for (int k = 0; k < PER16; ++k) e[k] = tile[ch * PER16 + k][cc];
-    *reinterpret_cast<u32x4*>(dst + (size_t)(c0 + cc) * ldt + r0 + ch * PER16) = *reinterpret_cast<u32x4*>(e);
+    for (int k = 0; k < 4; ++k) e[k] = (unsigned)tile[ch * 8 + 2 * k][cc] | ((unsigned)tile[ch * 8 + 2 * k + 1][cc] << 16);
+    *reinterpret_cast<u32x4*>(dst + (size_t)(c0 + cc) * ldt + r0 + ch * 8) = u32x4{e[0], e[1], e[2], e[3]};
+  }
+}
+
+// The three bf16 planes of an fp32 matrix [M, N] (any stride and alignment), straight [3][M, Np] and / or transposed
+// [3][Nt, Mp], zeros in the padding.
+__global__ __launch_bounds__(256) void vx_planes_kernel(const float* __restrict__ src, unsigned short* __restrict__ dst, unsigned short* __restrict__ dst_t,
+                                                        int M, int N, long lds_, int Np, int Nt, int Mp) {
+  __shared__ float tile[64][65];
+  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int rr = ty + 4 * i;
+    tile[rr][tx] = r0 + rr < M && c0 + tx < N ? src[(size_t)(r0 + rr) * lds_ + c0 + tx] : 0.f;
+  }
+  __syncthreads();
+  const int ch = threadIdx.x & 7, line = threadIdx.x >> 3;          // 8 elements of a row of the result
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    unsigned short* const out = turn ? dst_t : dst;
+    if (!out) continue;
+    const long ld = turn ? Mp : Np, lines = turn ? Nt : M, plane = lines * ld;
+    const int at = (turn ? r0 : c0) + ch * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int l = line + 32 * i, row = (turn ? c0 : r0) + l;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = turn ? tile[ch * 8 + k][l] : tile[l][ch * 8 + k];
+      if (row < lines && at < ld) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          unsigned e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned short lo = tk_f2bf(v[2 * k]), hi = tk_f2bf(v[2 * k + 1]);
+            e[k] = (unsigned)lo | ((unsigned)hi << 16);
+            const float dl = v[2 * k] - tk_bf2f(lo), dh = v[2 * k + 1] - tk_bf2f(hi);
+            v[2 * k] = fabsf(dl) < __builtin_huge_valf() ? dl : 0.f;
+            v[2 * k + 1] = fabsf(dh) < __builtin_huge_valf() ? dh : 0.f;
+          }
+          *reinterpret_cast<u32x4*>(out + q * plane + row * ld + at) = u32x4{e[0], e[1], e[2], e[3]};
+        }
+      }
+    }
   }
 }
 
@@ -519,65 +567,78 @@ __global__ __launch_bounds__(256) void vx_total_kernel(VxJoin a) {
 // --------------------------------------------------------------------------------------------------------- host side
 long up(long v, long to) { return (v + to - 1) / to * to; }
 
-// 256x256 blocks of the 8-wave kernel where they fill the chip (its staging offsets ask for whole half-tiles in range)
-bool use_pp(int dtype, long m, long n, long k, int splits) {
-  return dtype == TK_BF16 && m >= 256 && n >= 256 && k / splits >= 256 && ((m + 255) / 256) * ((n + 255) / 256) * splits >= 192;
+// 256x256 blocks of the 8-wave kernel (its staging offsets ask for whole half-tiles in range): one block a CU at 1300 TFLOP/s
+// of the whole chip against 450-600 of the 128x128 blocks, so from about 7/16 of the CUs on if the K loop is deep, from 3/4
+// on else.
+bool use_pp(int planes, long m, long n, long k, int splits) {
+  const long blocks = ((m + 255) / 256) * ((n + 255) / 256) * splits, deep = k / splits * (planes == 3 ? 6 : 1);
+  return m >= 256 && n >= 256 && k / splits >= 256 && blocks >= (deep >= 2048 ? 112 : 192);
 }
 
 // 128x128 blocks would leave most CUs idle, or their rows mostly empty
 bool use_skinny(long m, long n) { return m <= 16 || ((m + 127) / 128) * ((n + 127) / 128) < 128; }
 
 // Rows of a wave's block in the logits' epilogue
-int wave_rows(const VxGemm& a) { return use_skinny(a.M, a.N) ? 16 : use_pp(a.dtype, a.M, a.N, a.K, 1) ? 128 : 64; }
+int wave_rows(const VxGemm& a, bool skinny) { return skinny ? 16 : use_pp(a.a_plane ? 3 : 1, a.M, a.N, a.K, 1) ? 128 : 64; }
 
 template <int EPI>
 void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
-  if (use_pp(a.dtype, a.M, a.N, a.K, splits)) {
+  const bool planes = a.a_plane > 0;
+  if (use_pp(planes ? 3 : 1, a.M, a.N, a.K, splits)) {
     const dim3 g(dtf_cdiv(a.M, 256) * dtf_cdiv(a.N, 256), splits);
-    hipLaunchKernelGGL((gemm_pp_kernel<EPI, VxGemm>), g, dim3(512), 0, s, a);
+    if (planes) hipLaunchKernelGGL((gemm_pp_kernel<EPI + EPI_PLANES, VxGemm>), g, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((gemm_pp_kernel<EPI, VxGemm>), g, dim3(512), 0, s, a);
   } else {
     const dim3 g(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128), splits);
-    if (a.dtype == TK_BF16) hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, EPI, 4, 4, VxGemm>), g, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((gemm_tiled_kernel<unsigned int, EPI, 4, 4, VxGemm>), g, dim3(256), 0, s, a);
+    if (planes) hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, EPI + EPI_PLANES, 4, 4, VxGemm>), g, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, EPI, 4, 4, VxGemm>), g, dim3(256), 0, s, a);
   }
 }
 
 template <int EPI>
-void launch_logits(const VxGemm& a, hipStream_t s) {
-  if (!use_skinny(a.M, a.N)) return launch_gemm<EPI>(a, 1, s);
+void launch_logits(const VxGemm& a, bool skinny, hipStream_t s) {
+  if (!skinny) return launch_gemm<EPI>(a, 1, s);
   const dim3 g((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64)));
   if (a.dtype == TK_BF16) hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI>), g, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI>), g, dim3(256), 0, s, a);
 }
 
-VxGemm operands(const void* A, const void* B, int dtype, int M, int N, int K, long lda, long ldb) {
+// planes: 3 bf16 planes an operand, each dense; 1: the operands are of type dtype
+VxGemm operands(const void* A, const void* B, int dtype, int planes, int M, int N, int K, long lda, long ldb) {
   VxGemm g = {};
-  const long es = dtype == TK_BF16 ? 2 : 4;
+  const long es = planes == 3 || dtype == TK_BF16 ? 2 : 4;
   g.A = A; g.B = B; g.M = M; g.N = N; g.K = K;
   g.lda = (int)lda; g.ldb = (int)ldb; g.dtype = dtype;
-  g.a_bytes = (unsigned)(((M - 1) * lda + K) * es);
-  g.b_bytes = (unsigned)(((N - 1) * ldb + K) * es);
+  if (planes == 3) {
+    g.a_plane = (unsigned)(M * lda * es);
+    g.b_plane = (unsigned)(N * ldb * es);
+  }
+  g.a_bytes = 2 * g.a_plane + (unsigned)(((M - 1) * lda + K) * es);
+  g.b_bytes = 2 * g.b_plane + (unsigned)(((N - 1) * ldb + K) * es);
   return g;
 }
 
 // How many K ranges a product is cut into, so that its blocks fill the chip: 256x256 blocks (one a CU) if they do with
-// ranges of 1024 or more, else 128x128 blocks (two a CU), at least 512 deep.
-int splits_for(int dtype, long m, long n, long k) {
-  if (dtype == TK_BF16 && m >= 256 && n >= 256) {
+// ranges of 1024 or more, else 128x128 blocks (two a CU), at least 512 deep.  Planes make every range six times as deep.
+int splits_for(int planes, long m, long n, long k) {
+  const long deep = planes == 3 ? 128 : 512;
+  if (m >= 256 && n >= 256) {
     const long big = ((m + 255) / 256) * ((n + 255) / 256), s = std::max<long>(1, 256 / big);
-    if (big * s >= 192 && k / s >= 1024) return (int)s;
+    if (big * s >= 192 && k / s >= std::max<long>(256, 2 * deep)) return (int)s;
   }
   const long blocks = ((m + 127) / 128) * ((n + 127) / 128);
-  return (int)std::max<long>(1, std::min<long>({512 / blocks, k / 512, 32}));
+  return (int)std::max<long>(1, std::min<long>({512 / blocks, k / deep, 32}));
 }
 long kper_for(long k, int splits) { return up((k + splits - 1) / splits, 128); }
 
 // Sizes of one call: the padded width, the vocabulary piece and the workspace's parts
 struct VxPlan {
-  long es, per16, Dp, Np, Vp, pieces, strips, blocks;
-  bool pack_x, pack_w, direct_dx, direct_dw;
+  long Dp, Np, Vp, pieces, strips, blocks;
+  int K;                                         // of the logits: padded only where both operands are
+  int planes;                                    // of every operand of the large products
+  bool skinny, pack_x, pack_w, direct_dx, direct_dw;
   int sx, sw;                                    // splits of the two products
-  size_t x, w, part, target, blk, rows, xt, wt, dz, dzt, dx32, dw32, db, total;
+  size_t x, w, part, target, blk, rows, xt, wt, dz32, dz, dzt, dx32, dw32, db, total;
 };
 
 size_t take(size_t& at, size_t bytes) {
@@ -588,23 +649,30 @@ size_t take(size_t& at, size_t bytes) {
 
 VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   VxPlan p = {};
-  p.es = a.dtype == TK_BF16 ? 2 : 4;
-  p.per16 = 16 / p.es;
-  p.Dp = up(a.D, p.per16);
+  const long es = a.dtype == TK_BF16 ? 2 : 4, per16 = 16 / es;
+  p.planes = a.dtype == TK_BF16 ? 1 : 3;
+  p.Dp = up(a.D, 8);
   p.Np = up(a.N, 8);
-  p.pack_x = a.D % p.per16 || a.ldx % p.per16 || !dtf_aligned16(a.X);
-  p.pack_w = a.w_dtype != a.dtype || a.D % p.per16 || a.ldw % p.per16 || !dtf_aligned16(a.W);
   // a piece: dz and its transpose in 1 GiB, but never under 16384 columns (the products' K and M); every operand of a
   // launch stays below 2 GiB (32-bit offsets)
-  long vp = backward ? std::max<long>((1l << 30) / (2 * p.es * p.Np), 16384) : (1l << 30);
-  vp = std::min(vp, ((1l << 31) - (1 << 20)) / (p.es * std::max(p.Dp, backward ? p.Np : 0)));
+  const long col = 2 * p.planes;                 // bytes an element of an operand takes
+  long vp = backward ? std::max<long>((1l << 30) / (2 * col * p.Np), 16384) : (1l << 30);
+  vp = std::min(vp, ((1l << 31) - (1 << 20)) / (col * std::max(p.Dp, backward ? p.Np : 0)));
   vp = std::max<long>(vp / 256 * 256, 256);
   p.pieces = (a.V + vp - 1) / vp;
   p.Vp = p.pieces == 1 ? a.V : std::min(vp, up((a.V + p.pieces - 1) / p.pieces, 256));
   p.pieces = (a.V + p.Vp - 1) / p.Vp;
+  p.skinny = use_skinny(a.N, p.Vp);
+  // copies: bf16 where the operand's rows are no whole aligned 16-byte pieces; fp32 the same for the skinny kernel, planes
+  // for the others
+  const bool odd_x = a.D % per16 || a.ldx % per16 || !dtf_aligned16(a.X), odd_w = a.D % per16 || a.ldw % per16 || !dtf_aligned16(a.W);
+  p.K = p.skinny && a.D % per16 == 0 ? a.D : (int)p.Dp;
+  p.pack_x = p.planes == 3 && !p.skinny ? true : odd_x;
+  p.pack_w = p.planes == 3 && !p.skinny ? true : odd_w || a.w_dtype != a.dtype;
+  const size_t copy = p.planes == 3 && !p.skinny ? 6 : es;
   size_t at = 0;
-  if (p.pack_x) p.x = take(at, (size_t)a.N * p.Dp * p.es);
-  if (p.pack_w) p.w = take(at, (size_t)p.Vp * p.Dp * p.es);
+  if (p.pack_x) p.x = take(at, (size_t)a.N * p.Dp * copy);
+  if (p.pack_w) p.w = take(at, (size_t)p.Vp * p.Dp * copy);
   if (!backward) {
     p.strips = (a.V + kStrip - 1) / kStrip;
     p.blocks = (a.N + 63) / 64;
@@ -614,12 +682,13 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   } else {
     const long Vpp = up(p.Vp, 8);
     p.rows = take(at, (size_t)up(a.N, 256) * sizeof(VxRow) + 16);     // and the common factor behind them
-    p.xt = take(at, (size_t)p.Dp * p.Np * p.es);
-    p.wt = take(at, (size_t)p.Dp * Vpp * p.es);
-    p.dz = take(at, (size_t)a.N * Vpp * p.es);
-    p.dzt = take(at, (size_t)p.Vp * p.Np * p.es);
-    p.sx = splits_for(a.dtype, a.N, p.Dp, Vpp);
-    p.sw = splits_for(a.dtype, p.Vp, p.Dp, p.Np);
+    p.xt = take(at, (size_t)p.Dp * p.Np * col);
+    p.wt = take(at, (size_t)p.Dp * Vpp * col);
+    if (p.planes == 3) p.dz32 = take(at, (size_t)a.N * Vpp * 4);
+    p.dz = take(at, (size_t)a.N * Vpp * col);
+    p.dzt = take(at, (size_t)p.Vp * p.Np * col);
+    p.sx = splits_for(p.planes, a.N, p.Dp, Vpp);
+    p.sw = splits_for(p.planes, p.Vp, p.Dp, p.Np);
     p.sx = (int)((Vpp + kper_for(Vpp, p.sx) - 1) / kper_for(Vpp, p.sx));
     p.sw = (int)((p.Np + kper_for(p.Np, p.sw) - 1) / kper_for(p.Np, p.sw));
     // straight into the result where one product (or the last piece's) holds the whole sum at a 16-byte row width
@@ -654,12 +723,34 @@ void pack(const void* src, int sdt, void* dst, int ddt, long rows, int cols, lon
   else pack_as<unsigned short, unsigned short>(src, dst, rows, cols, lds_, ldd, s);
 }
 
-void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, int dtype, hipStream_t s) {
+void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, hipStream_t s) {
   const dim3 g((unsigned)((N + 63) / 64), (unsigned)((ldt + 63) / 64));
-  if (dtype == TK_BF16)
-    hipLaunchKernelGGL((vx_transpose_kernel<unsigned short>), g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt);
-  else
-    hipLaunchKernelGGL((vx_transpose_kernel<float>), g, dim3(256), 0, s, static_cast<const float*>(src), static_cast<float*>(dst), (int)M, (int)N, lds_, (int)ldt);
+  hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt);
+}
+
+void planes(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, hipStream_t s) {
+  const dim3 g((unsigned)((Np + 63) / 64), (unsigned)((Mp + 63) / 64));
+  hipLaunchKernelGGL(vx_planes_kernel, g, dim3(256), 0, s, static_cast<const float*>(src), static_cast<unsigned short*>(dst), static_cast<unsigned short*>(dst_t),
+                     (int)M, (int)N, lds_, (int)Np, (int)Nt, (int)Mp);
+}
+
+// One operand of the logits ([rows, D] of `from`, ld apart) as the kernel reads it, and transposed for a product (bf16: from
+// the aligned copy; to_t null: not needed).
+struct Operand { const void* p; long ld; };
+Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int from, long rows, long ld, bool copy, void* dst, void* to_t, long ldt, hipStream_t s) {
+  Operand o = {src, ld};
+  if (p.planes == 3) {
+    if (!p.skinny || to_t) planes(src, p.skinny ? nullptr : dst, to_t, rows, a.D, ld, p.Dp, p.Dp, ldt ? ldt : up(rows, 8), s);
+    if (p.skinny && copy) pack(src, from, dst, TK_F32, rows, a.D, ld, p.Dp, s);
+    if (!p.skinny || copy) o = {dst, p.Dp};
+  } else {
+    if (copy) {
+      pack(src, from, dst, TK_BF16, rows, a.D, ld, p.Dp, s);
+      o = {dst, p.Dp};
+    }
+    if (to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, s);
+  }
+  return o;
 }
 
 int check(const DtfVocabXentArgs* a) {
@@ -667,7 +758,7 @@ int check(const DtfVocabXentArgs* a) {
   if ((a->dtype != TK_F32 && a->dtype != TK_BF16) || (a->w_dtype != TK_F32 && a->w_dtype != TK_BF16)) return DTF_ERR_ARG;
   if (a->w_dtype == TK_BF16 && a->dtype == TK_F32) return DTF_ERR_ARG;
   if (a->N <= 0 || a->V <= 0 || a->D <= 0 || a->ldx < a->D || a->ldw < a->D) return DTF_ERR_SHAPE;
-  const long es = a->dtype == TK_BF16 ? 2 : 4, limit = (1l << 31) - (1 << 20);
+  const long es = a->dtype == TK_BF16 ? 2 : 6, limit = (1l << 31) - (1 << 20);          // fp32: three bf16 planes
   if (a->V > (1l << 30) || a->N > (1l << 26) || a->D > (1l << 20)) return DTF_ERR_SHAPE;
   if ((long)a->N * std::max<long>(a->ldx, up(a->D, 8)) * es > limit || (long)up(a->D, 8) * 256 * es > limit || (long)up(a->N, 8) * 256 * es > limit) return DTF_ERR_SHAPE;
   if (a->ldw > limit / (256 * es)) return DTF_ERR_SHAPE;
@@ -687,29 +778,18 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const void* X = a.X;
-  long ldx = a.ldx;
-  if (p.pack_x) {
-    pack(a.X, a.dtype, ws + p.x, a.dtype, a.N, a.D, a.ldx, p.Dp, s);
-    X = ws + p.x;
-    ldx = p.Dp;
-  }
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, nullptr, 0, s);
+  const int large = p.skinny ? 1 : p.planes;     // planes of the logits' operands
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0);
-    const void* W = static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4);
-    long ldw = a.ldw;
-    if (p.pack_w) {
-      pack(W, a.w_dtype, ws + p.w, a.dtype, n, a.D, a.ldw, p.Dp, s);
-      W = ws + p.w;
-      ldw = p.Dp;
-    }
-    VxGemm g = operands(X, W, a.dtype, a.N, (int)n, (int)p.Dp, ldx, ldw);
+    const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w, nullptr, 0, s);
+    VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.labels = a.labels;
     g.part = reinterpret_cast<float2*>(ws + p.part);
     g.target = reinterpret_cast<float2*>(ws + p.target);
     g.v0 = (int)v0;
-    launch_logits<VX_LSE>(g, s);
+    launch_logits<VX_LSE>(g, p.skinny, s);
   }
   VxJoin j = {reinterpret_cast<const float2*>(ws + p.part), reinterpret_cast<const float2*>(ws + p.target), a.labels, a.lse, a.loss_rows, a.loss,
               a.counts, reinterpret_cast<float*>(ws + p.blk), reinterpret_cast<int*>(ws + p.blk + p.blocks * 4), a.N, (int)p.strips, (int)p.blocks,
@@ -727,45 +807,34 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const void* X = a.X;
-  long ldx = a.ldx;
-  if (p.pack_x) {
-    pack(a.X, a.dtype, ws + p.x, a.dtype, a.N, a.D, a.ldx, p.Dp, s);
-    X = ws + p.x;
-    ldx = p.Dp;
-  }
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW ? ws + p.xt : nullptr, p.Np, s);
+  const int large = p.skinny ? 1 : p.planes;     // planes of the logits' operands
   VxRow* const rows = reinterpret_cast<VxRow*>(ws + p.rows);
   const int Mp = (int)up(a.N, 256);
   float* const scale = reinterpret_cast<float*>(rows + Mp);
   hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.lse, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, rows, scale);
-  if (a.dW) transpose(X, ws + p.xt, a.N, p.Dp, ldx, p.Np, a.dtype, s);
   float* const dx32 = reinterpret_cast<float*>(ws + p.dx32);
   float* const dw32 = reinterpret_cast<float*>(ws + p.dw32);
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0), np = up(n, 8);
-    const void* W = static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4);
-    long ldw = a.ldw;
-    if (p.pack_w) {
-      pack(W, a.w_dtype, ws + p.w, a.dtype, n, a.D, a.ldw, p.Dp, s);
-      W = ws + p.w;
-      ldw = p.Dp;
-    }
-    VxGemm g = operands(X, W, a.dtype, a.N, (int)n, (int)p.Dp, ldx, ldw);
+    const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w,
+                              a.dX ? ws + p.wt : nullptr, np, s);
+    VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.rows = rows;
     g.v0 = (int)v0;
-    g.C = ws + p.dz;
+    g.C = ws + (p.planes == 3 ? p.dz32 : p.dz);
     g.ldc = (int)np;
     g.Ct = ws + p.dzt;
     g.ldct = (int)p.Np;
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
-    launch_logits<VX_DZ>(g, s);
+    launch_logits<VX_DZ>(g, p.skinny, s);
+    if (p.planes == 3) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, np, np, n, p.Np, s);
     if (a.dbias) {
-      hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g)), (int)n, a.dbias + v0, scale);
+      hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
     }
     if (a.dX) {
-      transpose(W, ws + p.wt, n, p.Dp, ldw, np, a.dtype, s);
-      VxGemm d = operands(ws + p.dz, ws + p.wt, a.dtype, a.N, (int)p.Dp, (int)np, np, np);
+      VxGemm d = operands(ws + p.dz, ws + p.wt, TK_BF16, p.planes, a.N, (int)p.Dp, (int)np, np, np);
       const long kper = kper_for(up(p.Vp, 8), p.sx);
       const int splits = (int)((np + kper - 1) / kper);
       d.kper = p.sx > 1 ? (int)kper : 0;
@@ -780,7 +849,7 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
       launch_gemm<VX_SUM>(d, splits, s);
     }
     if (a.dW) {
-      VxGemm d = operands(ws + p.dzt, ws + p.xt, a.dtype, (int)n, (int)p.Dp, (int)p.Np, p.Np, p.Np);
+      VxGemm d = operands(ws + p.dzt, ws + p.xt, TK_BF16, p.planes, (int)n, (int)p.Dp, (int)p.Np, p.Np, p.Np);
       d.kper = p.sw > 1 ? (int)kper_for(p.Np, p.sw) : 0;
       void* const out = static_cast<char*>(a.dW) + v0 * a.D * (a.w_dtype == TK_BF16 ? 2 : 4);
       d.C32 = p.direct_dw && a.w_dtype == TK_F32 ? static_cast<float*>(out) : dw32;
