@@ -126,12 +126,16 @@ def vocab_xent_fwd(features: torch.Tensor, weight: torch.Tensor, labels: torch.T
     if reduction not in REDUCTIONS:
         raise ValueError(f"vocab_xent: reduction must be one of {REDUCTIONS}, got {reduction!r}")
     n, dev = features.shape[0], features.device
-    if not features.is_cuda or n == 0:
+    if n == 0:
+        _check(features, weight, labels, bias)
+        none = features.new_zeros(0, dtype=torch.float32)
+        return VocabXentResult(features.new_zeros((), dtype=torch.float32), none, none, labels.new_zeros(2), reduction, ignore_index)
+    if not features.is_cuda:
         _check(features, weight, labels, bias)
         return VocabXentResult(*reference.vocab_xent(features, weight, labels, bias, ignore_index, reduction), reduction, ignore_index)
-    rows = torch.empty((2, n), dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    counts = torch.empty(2, dtype=torch.int64, device=dev)
+    rows = features.new_empty((2, n), dtype=torch.float32)
+    loss = features.new_empty((), dtype=torch.float32)
+    counts = features.new_empty(2, dtype=torch.int64)
     a, keep = _build(features, weight, labels, bias, rows[1], counts, ignore_index, reduction == "mean")
     a.loss_rows, a.loss = rows.data_ptr(), loss.data_ptr()
     ws = _workspace(a, 0, dev)
@@ -152,7 +156,11 @@ def vocab_xent_bwd(fwd: VocabXentResult, features: torch.Tensor, weight: torch.T
     same_device("vocab_xent_bwd", features, dloss, fwd.lse)
     if fwd.lse.shape[0] != n:
         raise ValueError("vocab_xent_bwd: the forward result belongs to another batch")
-    if not features.is_cuda or n == 0:
+    if n == 0:
+        _check(features, weight, labels, bias)
+        return (torch.zeros_like(features) if want_x else None, weight.new_zeros(weight.shape) if want_w else None,
+                bias.new_zeros(bias.shape) if want_b else None)
+    if not features.is_cuda:
         _check(features, weight, labels, bias)
         d = reference.vocab_xent_bwd(features, weight, labels, bias, fwd.lse, fwd.counts, fwd.ignore_index, fwd.reduction, dloss)
         return d[0] if want_x else None, d[1] if want_w else None, d[2] if want_b else None

@@ -1,0 +1,163 @@
+"""The token-model operators as a model uses them: embedding -> dropout + residual -> layer norm -> hidden layer -> layer norm
+-> vocabulary head tied to the embedding table; gradients against 64 bits, training by the flat optimizer, a captured step."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from distributed_tensorflow_amd import ops
+from distributed_tensorflow_amd.ops.dropout import FusedDropout
+from distributed_tensorflow_amd.ops.embedding import ScaledEmbedding
+from distributed_tensorflow_amd.ops.layernorm import FusedLayerNorm
+from distributed_tensorflow_amd.ops.reference import dropout_mask
+from distributed_tensorflow_amd.ops.vocab_xent import vocab_xent
+from token_utils import U32, assert_within, devices
+
+V, D, T, RATE, PAD = 211, 40, 60, 0.25, 0
+
+
+class TextModel(nn.Module):
+    """Next-token classifier with one hidden block; the head's weight is the embedding table."""
+
+    def __init__(self):
+        super().__init__()
+        self.embed = ScaledEmbedding(V, D, scale=math.sqrt(D), padding_idx=PAD)
+        self.drop1, self.drop2 = FusedDropout(RATE, seed=1), FusedDropout(RATE, seed=2)
+        self.norm1, self.norm2 = FusedLayerNorm(D), FusedLayerNorm(D)
+        self.hidden = nn.Linear(D, D)
+        self.bias = nn.Parameter(torch.zeros(V))
+        with torch.no_grad():
+            self.embed.weight.normal_(0, 1 / math.sqrt(D))
+
+    def forward(self, ids, labels):
+        x = self.drop1(self.embed(ids))
+        h = self.norm1(x)
+        y, _ = self.norm2(self.drop2(torch.relu(self.hidden(h))), x)
+        return vocab_xent(y.reshape(-1, D), self.embed.weight, labels.reshape(-1), self.bias, ignore_index=PAD)
+
+
+def data(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(1, V, (3, T // 3), generator=g)
+    ids[2, -5:] = PAD
+    labels = torch.roll(ids, -1, 1)
+    return ids, labels
+
+
+def exact_loss(params, ids, labels, step):
+    """The same model in float64 with the same masks, by PyTorch's autograd."""
+    w, g1, b1, g2, b2, hw, hb, bias = params
+    keep = [dropout_mask((*ids.shape, D), RATE, s, step).double() * (65536 / (65536 - round(RATE * 65536))) for s in (1, 2)]
+    table = torch.where((torch.arange(V) == PAD)[:, None], w.detach(), w)      # no gradient through padding look-ups
+    x = table[ids] * math.sqrt(D) * keep[0]
+    norm = lambda t, g, b: nn.functional.layer_norm(t, (D,), g, b)  # noqa: E731
+    a = torch.relu(norm(x, g1, b1) @ hw.t() + hb) * keep[1]
+    z = (norm(a + x, g2, b2) @ w.t() + bias).reshape(-1, V)
+    return nn.functional.cross_entropy(z, labels.reshape(-1), ignore_index=PAD)
+
+
+def parameters(m):
+    return [m.embed.weight, m.norm1.weight, m.norm1.bias, m.norm2.weight, m.norm2.bias, m.hidden.weight, m.hidden.bias, m.bias]
+
+
+@pytest.mark.parametrize("dev", devices())
+def test_gradients_of_the_whole_model(dev):
+    torch.manual_seed(5)
+    m = TextModel().to(dev)
+    ids, labels = data()
+    for step in range(2):                                    # the second step draws other masks
+        m.zero_grad()
+        loss, hits = m(ids.to(dev), labels.to(dev))
+        loss.backward()
+        leaves = [p.detach().cpu().double().requires_grad_(True) for p in parameters(m)]
+        want = exact_loss(leaves, ids, labels, step)
+        want.backward()
+        assert abs(float(loss.detach()) - float(want.detach())) < 2e-5
+        assert 0 <= int(hits) <= int((labels != PAD).sum())
+        for p, leaf in zip(parameters(m), leaves):
+            # a chain of eight operators on values of order one to ten: below 2000 roundings of the largest gradient
+            assert_within(p.grad, leaf.grad, 2000 * U32 * leaf.grad.abs().max())
+
+
+@pytest.mark.parametrize("dev", devices())
+def test_training_steps_with_the_frameworks_optimizer(dev):
+    """A few Adam steps of the framework on one flat buffer: runs, changes every tensor that has a gradient, no NaN."""
+    torch.manual_seed(6)
+    m = TextModel().to(dev)
+    ids, labels = (t.to(dev) for t in data(1))
+    ps = parameters(m)
+    for t in range(1, 4):
+        grads = torch.autograd.grad(m(ids, labels)[0], ps)
+        before = [p.detach().clone() for p in ps]
+        for p, g in zip(ps, grads):
+            if t == 1:
+                p.m, p.v = torch.zeros_like(p), torch.zeros_like(p)
+            ops.adam_apply(p.detach().view(-1), g.contiguous().view(-1), p.m.view(-1), p.v.view(-1), 1e-2, step=t)
+        assert all(torch.isfinite(p).all() and not torch.equal(p, q) for p, q in zip(ps, before))
+    assert int(m.drop1.step) == 3
+
+
+@pytest.mark.gpu
+def test_captured_step_replays_with_new_data_and_masks():
+    torch.manual_seed(7)
+    m = TextModel().cuda()
+    ids, labels = (t.cuda() for t in data(2))
+    ps = parameters(m)
+
+    def step():
+        loss, hits = m(ids, labels)
+        return [loss.detach(), hits, *torch.autograd.grad(loss, ps)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        new = data(10 + k)
+        ids.copy_(new[0])
+        labels.copy_(new[1])
+        m.drop1.step.fill_(k)
+        m.drop2.step.fill_(k)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        m.drop1.step.fill_(k)
+        m.drop2.step.fill_(k)
+        for a, b in zip(got, step()):
+            # own kernels repeat bit for bit; the hidden layer's library product may choose another order in a graph
+            assert_within(a, b.double(), 2000 * U32 * b.double().abs().max() if a.is_floating_point() else 0)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Two models on two streams, launched in turn without waiting: workspaces are not shared."""
+    torch.manual_seed(8)
+    models = [TextModel().cuda() for _ in range(2)]
+    batches = [tuple(t.cuda() for t in data(20 + k)) for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def grads(k):
+        loss, _ = models[k](*batches[k])
+        return [loss.detach(), *torch.autograd.grad(loss, parameters(models[k]))]
+    alone = []
+    for k in range(2):
+        alone.append([t.clone() for t in grads(k)])
+        models[k].drop1.step.zero_()
+        models[k].drop2.step.zero_()
+    torch.cuda.synchronize()
+    both = [None, None]
+    for _ in range(3):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                models[k].drop1.step.zero_()
+                models[k].drop2.step.zero_()
+                both[k] = grads(k)
+    torch.cuda.synchronize()
+    for k in range(2):
+        for a, b in zip(both[k], alone[k]):
+            assert_within(a, b.double(), 2000 * U32 * b.double().abs().max())
