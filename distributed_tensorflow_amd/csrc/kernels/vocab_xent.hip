@@ -34,19 +34,25 @@
 #include "gemm_tiled.h"
 #include "token_ops.h"
 
-#define DTF_ROR16(v, n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), 0x120 + (n), 0xf, 0xf, false))
-
 namespace {
 enum { VX_LSE = EPI_CUSTOM, VX_DZ = EPI_CUSTOM + 1, VX_SUM = EPI_CUSTOM + 2 };
 constexpr int kStrip = 64;                       // columns a wave reduces in the forward pass
 constexpr int kLseSplits = 16;                   // waves of the join that share a row's strips
 
-__device__ __forceinline__ float max16(float v) {
-  v = fmaxf(v, DTF_ROR16(v, 8)); v = fmaxf(v, DTF_ROR16(v, 4)); v = fmaxf(v, DTF_ROR16(v, 2)); v = fmaxf(v, DTF_ROR16(v, 1));
-  return v;
+// Reductions over a 16-lane row by rotations, one instruction a step: the rotation is an operand modifier where nothing
+// hangs on the old value (bound_ctrl).  The maximum runs on integers in the floats' order (a float maximum would first
+// quieten every rotated operand): negative floats have their magnitude bits flipped.
+#define VX_ROR(v, n) __builtin_amdgcn_update_dpp(0, (v), 0x120 + (n), 0xf, 0xf, true)
+__device__ __forceinline__ float max16(float f) {
+  int v = __builtin_bit_cast(int, f);
+  v ^= (v >> 31) & 0x7fffffff;
+  v = max(v, VX_ROR(v, 8)); v = max(v, VX_ROR(v, 4)); v = max(v, VX_ROR(v, 2)); v = max(v, VX_ROR(v, 1));
+  v ^= (v >> 31) & 0x7fffffff;
+  return __builtin_bit_cast(float, v);
 }
+#define VX_RORF(v, n) __builtin_bit_cast(float, VX_ROR(__builtin_bit_cast(int, (v)), n))
 __device__ __forceinline__ float sum16(float v) {
-  v += DTF_ROR16(v, 8); v += DTF_ROR16(v, 4); v += DTF_ROR16(v, 2); v += DTF_ROR16(v, 1);
+  v += VX_RORF(v, 8); v += VX_RORF(v, 4); v += VX_RORF(v, 2); v += VX_RORF(v, 1);
   return v;
 }
 
@@ -61,7 +67,7 @@ __device__ __forceinline__ void unrolled(F&& f) {
 }
 
 // What the backward pass needs of a row; rows past the last have g = 0.
-struct VxRow {
+struct alignas(16) VxRow {
   float lse, g;
   int label, pad;                                // label: -1 where the row has none
 };
@@ -111,14 +117,23 @@ struct VxGemm : DtfGemmArgs {
       return;
     }
     const float NEG_INF = -__builtin_huge_valf();
+    if (bias) {
 #pragma unroll
-    for (int cj = 0; cj < 4; ++cj) {
-      const int col = ccol + 16 * cj + fr;
-      const float b = bias && col < N ? bias[col] : 0.f;
+      for (int cj = 0; cj < 4; ++cj) {
+        const float b = ccol + 16 * cj + fr < N ? bias[ccol + 16 * cj + fr] : 0.f;
 #pragma unroll
-      for (int ri = 0; ri < RI; ++ri)
+        for (int ri = 0; ri < RI; ++ri)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[ri][cj][r] = col < N ? acc[ri][cj][r] + b : NEG_INF;
+          for (int r = 0; r < 4; ++r) acc[ri][cj][r] += b;
+      }
+    }
+    if (ccol + kStrip > N) {                     // only the vocabulary's last strip has columns that do not exist
+#pragma unroll
+      for (int cj = 0; cj < 4; ++cj)
+#pragma unroll
+        for (int ri = 0; ri < RI; ++ri)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[ri][cj][r] = ccol + 16 * cj + fr < N ? acc[ri][cj][r] : NEG_INF;
     }
     if constexpr (EPI == VX_LSE) {
       float2* const out = part + (size_t)((v0 + ccol) / kStrip) * M;
@@ -160,25 +175,46 @@ struct VxGemm : DtfGemmArgs {
         }
       });
     } else {
-      float db[4] = {0.f, 0.f, 0.f, 0.f};
+      // p = exp(z - lse); rows without a gradient have g = 0 and get zeros whatever p is (a padding row may hold anything)
+      // The wave's rows go through its LDS (the images below overwrite them) and are read four at a time, again where a label
+      // is found: held at once they would not fit beside the accumulators.
+      VxRow* const lrow = reinterpret_cast<VxRow*>(wl);
 #pragma unroll
-      for (int ri = 0; ri < RI; ++ri)
+      for (int k = 0; k < (16 * RI + 63) / 64; ++k)
+        if (64 * k + lane < 16 * RI) lrow[64 * k + lane] = rows[crow + 64 * k + lane];
+      bool any = false;                          // a row's label lies in one strip of V / 64
+#pragma unroll
+      for (int ri = 0; ri < RI; ++ri) {
+        asm volatile("" ::: "memory");           // keeps the compiler from reading all rows up front
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const VxRow row = rows[crow + 16 * ri + 4 * g + r];
-          const int lab = row.label - v0 - ccol - fr;
+          const VxRow row = lrow[16 * ri + 4 * g + r];
+          any |= (unsigned)(row.label - v0 - ccol) < (unsigned)kStrip;       // label -1: far below or above every strip
 #pragma unroll
-          for (int cj = 0; cj < 4; ++cj) {
-            const float p = __expf(acc[ri][cj][r] - row.lse) - (row.label >= 0 && lab == 16 * cj ? 1.f : 0.f);
-            const float v = row.g == 0.f || ccol + 16 * cj + fr >= N ? 0.f : p * row.g;
-            acc[ri][cj][r] = v;
-            db[cj] += v;
+          for (int cj = 0; cj < 4; ++cj) acc[ri][cj][r] = row.g == 0.f ? 0.f : __expf(acc[ri][cj][r] - row.lse) * row.g;
+        }
+      }
+      if (__ballot(any)) {
+#pragma unroll
+        for (int ri = 0; ri < RI; ++ri) {
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const VxRow row = lrow[16 * ri + 4 * g + r];
+            const int at = row.label - v0 - ccol - fr;
+#pragma unroll
+            for (int cj = 0; cj < 4; ++cj) acc[ri][cj][r] -= at == 16 * cj ? row.g : 0.f;
           }
         }
+      }
       if (db_part) {
 #pragma unroll
         for (int cj = 0; cj < 4; ++cj) {
-          float v = db[cj];
+          float v = 0.f;
+#pragma unroll
+          for (int ri = 0; ri < RI; ++ri)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v += acc[ri][cj][r];
           v += __shfl_xor(v, 16);
           v += __shfl_xor(v, 32);
           const int col = ccol + 16 * cj + fr;
@@ -230,16 +266,25 @@ struct VxGemm : DtfGemmArgs {
       const u32x4 v = *reinterpret_cast<const u32x4*>(&wl[col * CH * 16 + ((q ^ (col & (CH - 1))) << 4)]);
       if (ccol + col < N && crow + q * 8 < ldct) *reinterpret_cast<u32x4*>(&ct[(size_t)(ccol + col) * ldct + crow + q * 8]) = v;
     }
+    // straight image: neighbouring lanes swap halves, so that a lane holds two rows of two neighbouring columns and writes
+    // 32-bit pieces (even lanes rows 0 and 1 of the four, odd lanes rows 2 and 3)
+    const bool odd = fr & 1;
+    const unsigned lo_sel = odd ? 0x05040100u : 0x01000504u, hi_sel = odd ? 0x07060302u : 0x03020706u;
+    // row 16 ri + 4 g + {0, 2}, 16-byte chunk (2 cj + fr / 8) ^ (row / 4): ri adds 2048 bytes and flips bit 2 of the chunk
+    const unsigned at0 = (unsigned)(4 * g + (odd ? 2 : 0)) * 128u + (unsigned)(fr & 6) * 2u, ch0 = (unsigned)((fr >> 3) ^ g);
 #pragma unroll
-    for (int ri = 0; ri < RI; ++ri)
+    for (int cj = 0; cj < 4; ++cj) {
+      unsigned char* const even_ri = wl + at0 + ((ch0 ^ (2 * cj)) << 4);
+      unsigned char* const odd_ri = wl + at0 + ((ch0 ^ (2 * cj) ^ 4) << 4);
 #pragma unroll
-      for (int cj = 0; cj < 4; ++cj)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int R = 16 * ri + 4 * g + r, col = 16 * cj + fr;
-          const unsigned w32 = r < 2 ? pk[ri][cj].x : pk[ri][cj].y;
-          *reinterpret_cast<unsigned short*>(&wl[R * 128 + ((((col >> 3) ^ (R >> 2)) & 7) << 4) + (col & 7) * 2]) = (unsigned short)((r & 1) ? (w32 >> 16) : (w32 & 0xffff));
-        }
+      for (int ri = 0; ri < RI; ++ri) {
+        const unsigned send = odd ? pk[ri][cj].x : pk[ri][cj].y, own = odd ? pk[ri][cj].y : pk[ri][cj].x;
+        const unsigned got = (unsigned)__builtin_amdgcn_update_dpp(0, (int)send, 0xB1, 0xf, 0xf, true);     // lane ^ 1
+        unsigned* const at = reinterpret_cast<unsigned*>((ri & 1 ? odd_ri : even_ri) + 2048 * ri);
+        at[0] = __builtin_amdgcn_perm(own, got, lo_sel);
+        at[32] = __builtin_amdgcn_perm(own, got, hi_sel);
+      }
+    }
 #pragma unroll
     for (int it = 0; it < 2 * RI; ++it) {
       const int R = it * 8 + (lane >> 3), q = lane & 7;
@@ -633,7 +678,9 @@ long kper_for(long k, int splits) { return up((k + splits - 1) / splits, 128); }
 
 // Sizes of one call: the padded width, the vocabulary piece and the workspace's parts
 struct VxPlan {
-  long Dp, Np, Vp, pieces, strips, blocks;
+  // Dp, Np: width and token count padded to 16 bytes (the products' sizes).  Copies' rows are ld* apart, a multiple of 128
+  // bytes: rows that straddle cache lines cost twice the requests (dX at 4093 x 50001 x 1024: 432 us with rows of 50008)
+  long Dp, Np, Vp, pieces, strips, blocks, ldd, ldn, ldv;
   int K;                                         // of the logits: padded only where both operands are
   int planes;                                    // of every operand of the large products
   bool skinny, pack_x, pack_w, direct_dx, direct_dw;
@@ -653,15 +700,18 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.planes = a.dtype == TK_BF16 ? 1 : 3;
   p.Dp = up(a.D, 8);
   p.Np = up(a.N, 8);
+  p.ldd = up(a.D, 64);
+  p.ldn = up(a.N, 64);
   // a piece: dz and its transpose in 1 GiB, but never under 16384 columns (the products' K and M); every operand of a
   // launch stays below 2 GiB (32-bit offsets)
   const long col = 2 * p.planes;                 // bytes an element of an operand takes
-  long vp = backward ? std::max<long>((1l << 30) / (2 * col * p.Np), 16384) : (1l << 30);
-  vp = std::min(vp, ((1l << 31) - (1 << 20)) / (col * std::max(p.Dp, backward ? p.Np : 0)));
+  long vp = backward ? std::max<long>((1l << 30) / (2 * col * p.ldn), 16384) : (1l << 30);
+  vp = std::min(vp, ((1l << 31) - (1 << 20)) / (col * std::max(p.ldd, backward ? p.ldn : 0)));
   vp = std::max<long>(vp / 256 * 256, 256);
   p.pieces = (a.V + vp - 1) / vp;
   p.Vp = p.pieces == 1 ? a.V : std::min(vp, up((a.V + p.pieces - 1) / p.pieces, 256));
   p.pieces = (a.V + p.Vp - 1) / p.Vp;
+  p.ldv = up(p.Vp, 64);
   p.skinny = use_skinny(a.N, p.Vp);
   // copies: bf16 where the operand's rows are no whole aligned 16-byte pieces; fp32 the same for the skinny kernel, planes
   // for the others
@@ -671,8 +721,8 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.pack_w = p.planes == 3 && !p.skinny ? true : odd_w || a.w_dtype != a.dtype;
   const size_t copy = p.planes == 3 && !p.skinny ? 6 : es;
   size_t at = 0;
-  if (p.pack_x) p.x = take(at, (size_t)a.N * p.Dp * copy);
-  if (p.pack_w) p.w = take(at, (size_t)p.Vp * p.Dp * copy);
+  if (p.pack_x) p.x = take(at, (size_t)a.N * p.ldd * copy);
+  if (p.pack_w) p.w = take(at, (size_t)p.Vp * p.ldd * copy);
   if (!backward) {
     p.strips = (a.V + kStrip - 1) / kStrip;
     p.blocks = (a.N + 63) / 64;
@@ -682,11 +732,11 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   } else {
     const long Vpp = up(p.Vp, 8);
     p.rows = take(at, (size_t)up(a.N, 256) * sizeof(VxRow) + 16);     // and the common factor behind them
-    p.xt = take(at, (size_t)p.Dp * p.Np * col);
-    p.wt = take(at, (size_t)p.Dp * Vpp * col);
-    if (p.planes == 3) p.dz32 = take(at, (size_t)a.N * Vpp * 4);
-    p.dz = take(at, (size_t)a.N * Vpp * col);
-    p.dzt = take(at, (size_t)p.Vp * p.Np * col);
+    p.xt = take(at, (size_t)p.Dp * p.ldn * col);
+    p.wt = take(at, (size_t)p.Dp * p.ldv * col);
+    if (p.planes == 3) p.dz32 = take(at, (size_t)a.N * p.ldv * 4);
+    p.dz = take(at, (size_t)a.N * p.ldv * col);
+    p.dzt = take(at, (size_t)p.Vp * p.ldn * col);
     p.sx = splits_for(p.planes, a.N, p.Dp, Vpp);
     p.sw = splits_for(p.planes, p.Vp, p.Dp, p.Np);
     p.sx = (int)((Vpp + kper_for(Vpp, p.sx) - 1) / kper_for(Vpp, p.sx));
@@ -740,13 +790,13 @@ struct Operand { const void* p; long ld; };
 Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int from, long rows, long ld, bool copy, void* dst, void* to_t, long ldt, hipStream_t s) {
   Operand o = {src, ld};
   if (p.planes == 3) {
-    if (!p.skinny || to_t) planes(src, p.skinny ? nullptr : dst, to_t, rows, a.D, ld, p.Dp, p.Dp, ldt ? ldt : up(rows, 8), s);
-    if (p.skinny && copy) pack(src, from, dst, TK_F32, rows, a.D, ld, p.Dp, s);
-    if (!p.skinny || copy) o = {dst, p.Dp};
+    if (!p.skinny || to_t) planes(src, p.skinny ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), s);
+    if (p.skinny && copy) pack(src, from, dst, TK_F32, rows, a.D, ld, p.ldd, s);
+    if (!p.skinny || copy) o = {dst, p.ldd};
   } else {
     if (copy) {
-      pack(src, from, dst, TK_BF16, rows, a.D, ld, p.Dp, s);
-      o = {dst, p.Dp};
+      pack(src, from, dst, TK_BF16, rows, a.D, ld, p.ldd, s);
+      o = {dst, p.ldd};
     }
     if (to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, s);
   }
@@ -760,7 +810,7 @@ int check(const DtfVocabXentArgs* a) {
   if (a->N <= 0 || a->V <= 0 || a->D <= 0 || a->ldx < a->D || a->ldw < a->D) return DTF_ERR_SHAPE;
   const long es = a->dtype == TK_BF16 ? 2 : 6, limit = (1l << 31) - (1 << 20);          // fp32: three bf16 planes
   if (a->V > (1l << 30) || a->N > (1l << 26) || a->D > (1l << 20)) return DTF_ERR_SHAPE;
-  if ((long)a->N * std::max<long>(a->ldx, up(a->D, 8)) * es > limit || (long)up(a->D, 8) * 256 * es > limit || (long)up(a->N, 8) * 256 * es > limit) return DTF_ERR_SHAPE;
+  if (a->N * std::max<long>(a->ldx, up(a->D, 64)) * es > limit || up(a->D, 64) * 256 * es > limit || up(a->N, 64) * 256 * es > limit) return DTF_ERR_SHAPE;
   if (a->ldw > limit / (256 * es)) return DTF_ERR_SHAPE;
   return DTF_OK;
 }
@@ -807,7 +857,7 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW ? ws + p.xt : nullptr, p.Np, s);
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW ? ws + p.xt : nullptr, p.ldn, s);
   const int large = p.skinny ? 1 : p.planes;     // planes of the logits' operands
   VxRow* const rows = reinterpret_cast<VxRow*>(ws + p.rows);
   const int Mp = (int)up(a.N, 256);
@@ -816,25 +866,25 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   float* const dx32 = reinterpret_cast<float*>(ws + p.dx32);
   float* const dw32 = reinterpret_cast<float*>(ws + p.dw32);
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
-    const long n = std::min<long>(p.Vp, a.V - v0), np = up(n, 8);
+    const long n = std::min<long>(p.Vp, a.V - v0), np = up(n, 8), ldv = up(n, 64);
     const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w,
-                              a.dX ? ws + p.wt : nullptr, np, s);
+                              a.dX ? ws + p.wt : nullptr, ldv, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.rows = rows;
     g.v0 = (int)v0;
     g.C = ws + (p.planes == 3 ? p.dz32 : p.dz);
-    g.ldc = (int)np;
+    g.ldc = (int)ldv;
     g.Ct = ws + p.dzt;
-    g.ldct = (int)p.Np;
+    g.ldct = (int)p.ldn;
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
     launch_logits<VX_DZ>(g, p.skinny, s);
-    if (p.planes == 3) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, np, np, n, p.Np, s);
+    if (p.planes == 3) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, s);
     if (a.dbias) {
       hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
     }
     if (a.dX) {
-      VxGemm d = operands(ws + p.dz, ws + p.wt, TK_BF16, p.planes, a.N, (int)p.Dp, (int)np, np, np);
+      VxGemm d = operands(ws + p.dz, ws + p.wt, TK_BF16, p.planes, a.N, (int)p.Dp, (int)np, ldv, ldv);
       const long kper = kper_for(up(p.Vp, 8), p.sx);
       const int splits = (int)((np + kper - 1) / kper);
       d.kper = p.sx > 1 ? (int)kper : 0;
@@ -849,7 +899,7 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
       launch_gemm<VX_SUM>(d, splits, s);
     }
     if (a.dW) {
-      VxGemm d = operands(ws + p.dzt, ws + p.xt, TK_BF16, p.planes, (int)n, (int)p.Dp, (int)p.Np, p.Np, p.Np);
+      VxGemm d = operands(ws + p.dzt, ws + p.xt, TK_BF16, p.planes, (int)n, (int)p.Dp, (int)p.Np, p.ldn, p.ldn);
       d.kper = p.sw > 1 ? (int)kper_for(p.Np, p.sw) : 0;
       void* const out = static_cast<char*>(a.dW) + v0 * a.D * (a.w_dtype == TK_BF16 ? 2 : 4);
       d.C32 = p.direct_dw && a.w_dtype == TK_F32 ? static_cast<float*>(out) : dw32;
