@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
 DTF_EXPORT int dtf_dropout(const void* x, const void* res, void* y, int64_t n, int dtype, double rate, uint64_t seed, uint64_t step,
                            const long long* step_ptr, long long* used, hipStream_t s) {
   if (!(rate >= 0.0 && rate <= 1.0) || (dtype != TK_F32 && dtype != TK_BF16)) return DTF_ERR_ARG;
-  if (n < 0 || (n + 2047) / 2048 > 0x7fffffffLL) return DTF_ERR_SHAPE;
+  if (n < 0 || n >= (1ll << 35) - 4096) return DTF_ERR_SHAPE;         // fewer than 2^32 threads
   if (n > 0 && (!x || !y)) return DTF_ERR_ARG;
   if (n == 0 && !used) return DTF_OK;
   const unsigned thr = (unsigned)__builtin_rint(rate * 65536.0);     // ties to even, like Python's round

@@ -404,7 +404,7 @@ EmbPlan plan(int64_t n, int64_t V, int D) {
 
 int check(int64_t n, int64_t V, int64_t D, int dtype) {
   if (dtype != TK_F32 && dtype != TK_BF16) return DTF_ERR_ARG;
-  if (n < 0 || n > (1ll << 28) || V <= 0 || V > (1ll << 30) || D <= 0 || D > (1 << 20)) return DTF_ERR_SHAPE;
+  if (n < 0 || n > (1ll << 25) || V <= 0 || V > (1ll << 30) || D <= 0 || D > (1 << 20)) return DTF_ERR_SHAPE;
   return DTF_OK;
 }
 

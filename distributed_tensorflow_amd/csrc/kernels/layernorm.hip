@@ -68,7 +68,7 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LnArgs a) {
   constexpr int VEC = P::VEC;
   __shared__ float s_sum[2][1][kBlock / 64];
   const int t = threadIdx.x % TPR;
-  const long row = (long)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+  const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * (BLOCK / TPR) + threadIdx.x / TPR;
   const bool live = row < a.rows;            // dead rows of the last workgroup still take part in its barriers
   const T* const x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
   tk_u32x4 raw[NV];
@@ -153,7 +153,8 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(LnArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kBlock) void ln_fwd_stream_kernel(LnArgs a) {
   __shared__ float s_sum[2][1][kBlock / 64];
-  const long row = blockIdx.x;
+  const long row = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  if (row >= a.rows) return;
   const T* src = static_cast<const T*>(a.x) + row * a.ldx;
   const T* const r = a.res ? static_cast<const T*>(a.res) + row * a.ldres : nullptr;
   T* const h = a.res ? static_cast<T*>(a.h) + row * a.C : nullptr;
@@ -307,7 +308,8 @@ __global__ __launch_bounds__(kBwdBlock) void ln_bwd_kernel(LnBwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kBlock) void ln_bwd_stream_kernel(LnBwdArgs a) {
   __shared__ float s_sum[2][2][kBlock / 64];
-  const long row = blockIdx.x;
+  const long row = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  if (row >= a.rows) return;
   const T* const dy = static_cast<const T*>(a.dy) + row * a.lddy;
   const T* const h = static_cast<const T*>(a.h) + row * a.ldh;
   const T* const dh = a.dh ? static_cast<const T*>(a.dh) + row * a.lddh : nullptr;
@@ -372,11 +374,17 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
 
 bool vec_ok(const void* p, long ld, int vec, int es) { return !p || (((uintptr_t)p & 15) == 0 && ld % vec == 0 && vec * es == 16); }
 
+// `blocks` workgroups as a grid of two indices: a launch's x may not reach 2^32 threads
+dim3 grid2(long blocks) {
+  const long x = std::min<long>(blocks, 1 << 20);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+
 template <typename T, bool AL, int NV, int TPR>
 void fwd_as(const LnArgs& a, hipStream_t s) {
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
   const long rpb = BLOCK / TPR;
-  hipLaunchKernelGGL((ln_fwd_kernel<T, AL, NV, TPR, BLOCK>), dim3((unsigned)((a.rows + rpb - 1) / rpb)), dim3(BLOCK), 0, s, a);
+  hipLaunchKernelGGL((ln_fwd_kernel<T, AL, NV, TPR, BLOCK>), grid2((a.rows + rpb - 1) / rpb), dim3(BLOCK), 0, s, a);
 }
 
 template <typename T, bool AL>
@@ -387,7 +395,7 @@ void fwd_width(const LnArgs& a, hipStream_t s) {
   else if (a.C <= 256 * 16) fwd_as<T, AL, N16, 256>(a, s);
   else if (a.C <= 512 * 16) fwd_as<T, AL, N16, 512>(a, s);
   else if (a.C <= 1024 * 16) fwd_as<T, AL, N16, 1024>(a, s);
-  else hipLaunchKernelGGL((ln_fwd_stream_kernel<T>), dim3((unsigned)a.rows), dim3(kBlock), 0, s, a);
+  else hipLaunchKernelGGL((ln_fwd_stream_kernel<T>), grid2(a.rows), dim3(kBlock), 0, s, a);
 }
 
 int bwd_parts(long rows, int C) {
@@ -406,7 +414,7 @@ void bwd_width(const LnBwdArgs& a, int parts, hipStream_t s) {
   else if (a.C <= 512 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, N16, 512>), g, b, 0, s, a);
   else if (a.C <= 1024 * 16) hipLaunchKernelGGL((ln_bwd_kernel<T, AL, 2 * N16, 512>), g, b, 0, s, a);
   else {
-    hipLaunchKernelGGL((ln_bwd_stream_kernel<T>), dim3((unsigned)a.rows), dim3(kBlock), 0, s, a);
+    hipLaunchKernelGGL((ln_bwd_stream_kernel<T>), grid2(a.rows), dim3(kBlock), 0, s, a);
     if (a.want_wgrad) hipLaunchKernelGGL((ln_colsum_kernel<T>), dim3(dtf_cdiv(a.C, 256), parts), dim3(256), 0, s, a);
   }
 }

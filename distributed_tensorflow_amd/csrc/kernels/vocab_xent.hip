@@ -397,7 +397,7 @@ __global__ __launch_bounds__(256) void vx_pack_kernel(const TS* __restrict__ src
 // dst[c, r] = src[r, c] for r < M, c < N; zeros for r in [M, ldt).  64 x 64 tiles through LDS.
 __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short* __restrict__ src, unsigned short* __restrict__ dst, int M, int N, long lds_, int ldt) {
   __shared__ unsigned short tile[64][72];
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+  const int across = (N + 63) >> 6, c0 = (int)(blockIdx.x % across) * 64, r0 = (int)(blockIdx.x / across) * 64;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int id = threadIdx.x + 256 * i, rr = id >> 3, ch = id & 7;
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short*
 __global__ __launch_bounds__(256) void vx_planes_kernel(const float* __restrict__ src, unsigned short* __restrict__ dst, unsigned short* __restrict__ dst_t,
                                                         int M, int N, long lds_, int Np, int Nt, int Mp) {
   __shared__ float tile[64][65];
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int across = (Np + 63) >> 6, c0 = (int)(blockIdx.x % across) * 64, r0 = (int)(blockIdx.x / across) * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int rr = ty + 4 * i;
@@ -706,7 +706,7 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   // launch stays below 2 GiB (32-bit offsets)
   const long col = 2 * p.planes;                 // bytes an element of an operand takes
   long vp = backward ? std::max<long>((1l << 30) / (2 * col * p.ldn), 16384) : (1l << 30);
-  vp = std::min(vp, ((1l << 31) - (1 << 20)) / (col * std::max(p.ldd, backward ? p.ldn : 0)));
+  vp = std::min(vp, ((1l << 31) - (1 << 20)) / (col * std::max({p.ldd, (long)a.ldw, backward ? p.ldn : 0})));
   vp = std::max<long>(vp / 256 * 256, 256);
   p.pieces = (a.V + vp - 1) / vp;
   p.Vp = p.pieces == 1 ? a.V : std::min(vp, up((a.V + p.pieces - 1) / p.pieces, 256));
@@ -774,12 +774,12 @@ void pack(const void* src, int sdt, void* dst, int ddt, long rows, int cols, lon
 }
 
 void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, hipStream_t s) {
-  const dim3 g((unsigned)((N + 63) / 64), (unsigned)((ldt + 63) / 64));
+  const dim3 g((unsigned)(((N + 63) / 64) * ((ldt + 63) / 64)));            // one index: there may be more than 65535 tile rows
   hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt);
 }
 
 void planes(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, hipStream_t s) {
-  const dim3 g((unsigned)((Np + 63) / 64), (unsigned)((Mp + 63) / 64));
+  const dim3 g((unsigned)(((Np + 63) / 64) * ((Mp + 63) / 64)));
   hipLaunchKernelGGL(vx_planes_kernel, g, dim3(256), 0, s, static_cast<const float*>(src), static_cast<unsigned short*>(dst), static_cast<unsigned short*>(dst_t),
                      (int)M, (int)N, lds_, (int)Np, (int)Nt, (int)Mp);
 }
@@ -880,9 +880,8 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
     launch_logits<VX_DZ>(g, p.skinny, s);
     if (p.planes == 3) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, s);
-    if (a.dbias) {
+    if (a.dbias)
       hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
-    }
     if (a.dX) {
       VxGemm d = operands(ws + p.dz, ws + p.wt, TK_BF16, p.planes, a.N, (int)p.Dp, (int)np, ldv, ldv);
       const long kper = kper_for(up(p.Vp, 8), p.sx);

@@ -332,3 +332,44 @@ def test_same_bits_again_on_another_stream_and_in_replayed_graphs():
         want = step()
         for _, out in graphs:
             assert all(torch.equal(a, c) for a, c in zip(want, out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_millions_of_columns(dtype):
+    """More than 65535 tiles of 64 vocabulary rows."""
+    n, v, d = 2, 4_300_000, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, w = torch.randn((n, d), generator=g, device="cuda").to(dtype), torch.randn((v, d), generator=g, device="cuda").to(dtype)
+    lab = torch.tensor([17, v - 1], device="cuda")
+    r = vx.vocab_xent_fwd(x, w, lab)
+    dx, dw, _ = vx.vocab_xent_bwd(r, x, w, lab)
+    xd = x.double().requires_grad_(True)
+    wd = w.double().requires_grad_(True)
+    loss = torch.nn.functional.cross_entropy(xd @ wd.t(), lab)
+    loss.backward()
+    # sum |x w| stays below 60 here, so a logit is off by at most 10 U32 * 60 = 4e-5, lse by that and 150 U32, and a
+    # probability by 1e-4 of itself; both gradients are sums of terms dz x and dz w, bounded by 1e-4 (and the operands'
+    # rounding) of the sum of the terms' sizes, not of the sum, in which the rows' terms may cancel
+    assert float((xd.detach().abs() @ wd.detach().abs().t()).max()) < 60
+    assert abs(float(r.loss) - float(loss.detach())) < 1e-4
+    step = half_step(dtype)
+    dz = torch.softmax(xd.detach() @ wd.detach().t(), 1) / n
+    dz[torch.arange(n), lab] -= 1 / n
+    assert_within(dw, wd.grad, (2 * step + 1e-4) * (dz.abs().t() @ xd.detach().abs()))
+    assert_within(dx, xd.grad, (2 * step + 1e-4) * (dz.abs() @ wd.detach().abs()))
+
+
+@pytest.mark.gpu
+def test_weight_rows_so_far_apart_that_a_piece_must_be_shorter():
+    """40 000 rows 65 536 elements apart are 5 GB from end to end: beyond one launch's 32-bit offsets."""
+    x, w, lab, b = (t.cuda() for t in draw(50, 40000, 64, torch.bfloat16))
+    far = torch.zeros((40000, 65536), dtype=torch.bfloat16, device="cuda")[:, 256:320]
+    far.copy_(w)
+    # shorter pieces may run on another kernel, with another order of sums: held to the definition, not to the other's bits
+    want = exact(x, w, lab, b)
+    r = vx.vocab_xent_fwd(x, far, lab, b)
+    assert_within(r.loss_rows, *want["rows"], "loss rows")
+    assert int(r.hits) == want["hits"]
+    for got, name in zip(vx.vocab_xent_bwd(r, x, far, lab, b), ("dx", "dw", "db")):
+        assert_within(got, *want[name], name)

@@ -238,3 +238,17 @@ def test_same_bits_again_on_another_stream_and_in_a_replayed_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(step(), out))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_index_holds():
+    """70 million rows of four: a row takes a wave, and 2^32 threads are more than one grid dimension may have."""
+    rows = 70_000_001
+    x = torch.randint(-3, 4, (rows, 4), device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    r = ln.layer_norm_fwd(x)
+    dx, dw, db = ln.layer_norm_bwd(torch.ones_like(x), r)
+    for part in (slice(0, 1000), slice(1 << 26, (1 << 26) + 1000), slice(rows - 1000, rows)):
+        want = exact(x[part].cpu(), None, None)
+        assert_within(r.y[part], *want["y"], "y")
+    assert torch.equal(db, torch.full((4,), float(rows), device="cuda"))
+    assert dx.abs().max() < 1e-2                     # dy = 1: nothing but the rounding of sums of four is left
