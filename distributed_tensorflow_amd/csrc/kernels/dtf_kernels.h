@@ -513,14 +513,16 @@ DTF_EXPORT int dtf_upload_words(void* dst, const void* host_src, int64_t n_words
 DTF_EXPORT int dtf_kernels_abi_version();
 
 // Softmax cross entropy over a large vocabulary in pieces (vocab_xent.hip).  Forward reads X, W, labels, bias and writes
-// lse, loss_rows, loss, counts; backward reads those, and dloss, and writes dX [N, D], dW [V, D], dbias [V] (dense; null:
+// lse, top, total, loss_rows, loss, counts; backward reads top, total, counts and dloss, and writes dX [N, D], dW [V, D], dbias [V] (dense; null:
 // left out).
 struct DtfVocabXentArgs {
   const void* X;            // [N, ldx] of `dtype`
   const void* W;            // [V, ldw] of `w_dtype`: `dtype`, or fp32 under bf16 activations
   const float* bias;        // [V], optional
   const long long* labels;  // [N] class indices; `ignore`: a row without loss
-  float* lse;               // [N]
+  float* lse;               // [N] = top + log total
+  float* top;               // [N] the row's largest logit
+  float* total;             // [N] sum of exp(logit - top)
   float* loss_rows;         // [N]
   float* loss;              // [1] mean over the rows with a label, or sum
   long long* counts;        // [2] hits, rows with a label

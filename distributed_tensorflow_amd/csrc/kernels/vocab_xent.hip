@@ -1,7 +1,7 @@
 // Softmax cross entropy over a large vocabulary without keeping the logits: z = X W^T + b, X [N tokens, D], W [V, D].
 //
 //   forward    lse_r = log sum_c exp z_rc;   loss_r = lse_r - z_r,label;   hit_r: label is the first maximum of the row
-//   backward   dz_rc = (exp(z_rc - lse_r) - [c = label_r]) g_r;   dX = dz W;   dW = dz^T X;   db_c = sum_r dz_rc
+//   backward   dz_rc = (exp z_rc / sum_c exp z_rc - [c = label_r]) g_r;   dX = dz W;   dW = dz^T X;   db_c = sum_r dz_rc
 //
 // Forward: one GEMM whose epilogue reduces each row of a wave's 64-column strip to (maximum, sum of exponentials) and
 // picks the label's logit on the way; a join over the strips gives lse, loss and hits.  8 bytes a strip and row leave the
@@ -66,11 +66,21 @@ __device__ __forceinline__ void unrolled(F&& f) {
   }
 }
 
-// What the backward pass needs of a row; rows past the last have g = 0.
+// What the backward pass needs of a row: p = exp(z - top) / total, so dz = exp(z - top) scaled - [label] g with scaled = g /
+// total.  (exp(z - lse) would carry lse's own rounding, half a step of a value near 10, into every element of the row.)
+// Rows past the last and rows without a label have g = 0.
 struct alignas(16) VxRow {
-  float lse, g;
-  int label, pad;                                // label: -1 where the row has none
+  float top, scaled, g;
+  int label;                                     // -1 where the row has none
 };
+
+// exp(d) for d <= 0 or so with the rounding of d log2(e) made good: the product's error, up to |d| 2^-24 of the result, is
+// computed and applied to first order.
+__device__ __forceinline__ float exp_exact(float d) {
+  const float hi = d * 1.44269502f, lo = fmaf(d, 1.92596303e-8f, fmaf(d, 1.44269502f, -hi));
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return e > 0.f ? fmaf(e * 0.693147181f, lo, e) : e;              // 0 and NaN as they are
+}
 
 struct VxGemm : DtfGemmArgs {
   // VX_LSE
@@ -175,7 +185,7 @@ struct VxGemm : DtfGemmArgs {
         }
       });
     } else {
-      // p = exp(z - lse); rows without a gradient have g = 0 and get zeros whatever p is (a padding row may hold anything)
+      // rows without a gradient have g = 0 and get zeros whatever p is (a padding row may hold anything)
       // The wave's rows go through its LDS (the images below overwrite them) and are read four at a time, again where a label
       // is found: held at once they would not fit beside the accumulators.
       VxRow* const lrow = reinterpret_cast<VxRow*>(wl);
@@ -191,7 +201,10 @@ struct VxGemm : DtfGemmArgs {
           const VxRow row = lrow[16 * ri + 4 * g + r];
           any |= (unsigned)(row.label - v0 - ccol) < (unsigned)kStrip;       // label -1: far below or above every strip
 #pragma unroll
-          for (int cj = 0; cj < 4; ++cj) acc[ri][cj][r] = row.g == 0.f ? 0.f : __expf(acc[ri][cj][r] - row.lse) * row.g;
+          for (int cj = 0; cj < 4; ++cj) {
+            const float d = acc[ri][cj][r] - row.top;
+            acc[ri][cj][r] = row.g == 0.f ? 0.f : (F32 ? exp_exact(d) : __expf(d)) * row.scaled;
+          }
         }
       }
       if (__ballot(any)) {
@@ -489,7 +502,7 @@ __global__ __launch_bounds__(256) void vx_db_kernel(const float* __restrict__ pa
   db[c] = v * *scale;
 }
 
-__global__ __launch_bounds__(256) void vx_rows_kernel(const float* __restrict__ lse, const long long* __restrict__ labels, const float* __restrict__ dloss,
+__global__ __launch_bounds__(256) void vx_rows_kernel(const float* __restrict__ top, const float* __restrict__ total, const long long* __restrict__ labels, const float* __restrict__ dloss,
                                                       int dloss_rows, const long long* __restrict__ counts, int mean, int M, int Mp, long V,
                                                       long long ignore, VxRow* __restrict__ rows, float* __restrict__ scale) {
   const int r = blockIdx.x * 256 + threadIdx.x;
@@ -498,12 +511,13 @@ __global__ __launch_bounds__(256) void vx_rows_kernel(const float* __restrict__ 
     *scale = mean ? (counts[1] ? up / (float)counts[1] : 0.f) : up;
   }
   if (r >= Mp) return;
-  VxRow o = {0.f, 0.f, -1, 0};
+  VxRow o = {0.f, 0.f, 0.f, -1};
   if (r < M) {
     const long long lab = labels[r];
     if (lab != ignore && lab >= 0 && lab < V) {
-      o.lse = lse[r];
+      o.top = top[r];
       o.g = dloss_rows ? dloss[r] : 1.f;
+      o.scaled = o.g / total[r];
       o.label = (int)lab;
     }
   }
@@ -520,7 +534,7 @@ __device__ __forceinline__ void lse_add(float& m, float& s, float m2, float s2) 
 // 64 rows a workgroup, 16 waves share a row's strips.  block_out: this workgroup's sums, or (last = only workgroup) the result.
 struct VxJoin {
   const float2* part; const float2* target; const long long* labels;
-  float* lse; float* loss_rows; float* loss; long long* counts; float* blk_loss; int* blk_counts;
+  float* lse; float* top; float* total; float* loss_rows; float* loss; long long* counts; float* blk_loss; int* blk_counts;
   int M, strips, blocks, mean; long V; long long ignore;
 };
 
@@ -567,6 +581,8 @@ __global__ __launch_bounds__(64 * kLseSplits) void vx_join_kernel(VxJoin a) {
     const float lse = m + logf(s);
     const long long lab = a.labels[row];
     a.lse[row] = lse;
+    a.top[row] = m;
+    a.total[row] = s;
     if (lab != a.ignore) {
       valid = 1;
       if (lab >= 0 && lab < a.V) {
@@ -823,7 +839,7 @@ DTF_EXPORT int64_t dtf_vocab_xent_ws_bytes(const DtfVocabXentArgs* a, int backwa
 DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (const int rc = check(ap)) return rc;
   const DtfVocabXentArgs& a = *ap;
-  if (!a.X || !a.W || !a.labels || !a.lse || !a.loss_rows || !a.loss || !a.counts || !a.ws) return DTF_ERR_ARG;
+  if (!a.X || !a.W || !a.labels || !a.lse || !a.top || !a.total || !a.loss_rows || !a.loss || !a.counts || !a.ws) return DTF_ERR_ARG;
   const VxPlan p = plan(a, false);
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
@@ -841,7 +857,7 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.v0 = (int)v0;
     launch_logits<VX_LSE>(g, p.skinny, s);
   }
-  VxJoin j = {reinterpret_cast<const float2*>(ws + p.part), reinterpret_cast<const float2*>(ws + p.target), a.labels, a.lse, a.loss_rows, a.loss,
+  VxJoin j = {reinterpret_cast<const float2*>(ws + p.part), reinterpret_cast<const float2*>(ws + p.target), a.labels, a.lse, a.top, a.total, a.loss_rows, a.loss,
               a.counts, reinterpret_cast<float*>(ws + p.blk), reinterpret_cast<int*>(ws + p.blk + p.blocks * 4), a.N, (int)p.strips, (int)p.blocks,
               a.mean, a.V, a.ignore};
   hipLaunchKernelGGL(vx_join_kernel, dim3((unsigned)p.blocks), dim3(64 * kLseSplits), 0, s, j);
@@ -852,7 +868,7 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
 DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (const int rc = check(ap)) return rc;
   const DtfVocabXentArgs& a = *ap;
-  if (!a.X || !a.W || !a.labels || !a.lse || !a.counts || !a.ws || !(a.dX || a.dW || a.dbias)) return DTF_ERR_ARG;
+  if (!a.X || !a.W || !a.labels || !a.top || !a.total || !a.counts || !a.ws || !(a.dX || a.dW || a.dbias)) return DTF_ERR_ARG;
   const VxPlan p = plan(a, true);
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
@@ -862,7 +878,7 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   VxRow* const rows = reinterpret_cast<VxRow*>(ws + p.rows);
   const int Mp = (int)up(a.N, 256);
   float* const scale = reinterpret_cast<float*>(rows + Mp);
-  hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.lse, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, rows, scale);
+  hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.top, a.total, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, rows, scale);
   float* const dx32 = reinterpret_cast<float*>(ws + p.dx32);
   float* const dw32 = reinterpret_cast<float*>(ws + p.dw32);
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {

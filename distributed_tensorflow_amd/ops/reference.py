@@ -202,7 +202,8 @@ def _vocab_labels(labels, vocab, ignore_index):
 
 
 def vocab_xent(features, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
-    """``(loss, loss_rows, lse, [hits, rows with a label])`` of softmax cross entropy on ``features @ weight.T + bias``."""
+    """``(loss, rows, [hits, rows with a label])`` of softmax cross entropy on ``features @ weight.T + bias``; ``rows`` [4, N]:
+    loss, logarithm of the sum of exponentials, largest logit, sum of exponentials relative to it."""
     z = features.float() @ weight.float().t()
     if bias is not None:
         z = z + bias.float()
@@ -213,7 +214,8 @@ def vocab_xent(features, weight, labels, bias=None, ignore_index=-100, reduction
     total = rows.sum()
     if reduction == "mean":
         total = total / counts[1].clamp_min(1)
-    return total, rows, lse, counts
+    top = z.amax(1)
+    return total, torch.stack((rows, lse, top, torch.exp(z - top[:, None]).sum(1))), counts
 
 
 def vocab_xent_bwd(features, weight, labels, bias, lse, counts, ignore_index=-100, reduction="mean", dloss=None):

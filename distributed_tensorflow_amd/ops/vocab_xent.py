@@ -34,7 +34,7 @@ REDUCTIONS = ("mean", "sum", "none")
 class _Args(C.Structure):
     """Mirror of ``DtfVocabXentArgs``."""
     _fields_ = [("X", C.c_void_p), ("W", C.c_void_p), ("bias", C.c_void_p), ("labels", C.c_void_p), ("lse", C.c_void_p),
-                ("loss_rows", C.c_void_p), ("loss", C.c_void_p), ("counts", C.c_void_p), ("dloss", C.c_void_p),
+                ("top", C.c_void_p), ("total", C.c_void_p), ("loss_rows", C.c_void_p), ("loss", C.c_void_p), ("counts", C.c_void_p), ("dloss", C.c_void_p),
                 ("dX", C.c_void_p), ("dW", C.c_void_p), ("dbias", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
                 ("ignore", C.c_longlong), ("ldx", C.c_int64), ("ldw", C.c_int64), ("V", C.c_int64), ("N", C.c_int),
                 ("D", C.c_int), ("dtype", C.c_int), ("w_dtype", C.c_int), ("mean", C.c_int), ("dloss_rows", C.c_int)]
@@ -56,13 +56,22 @@ def _kernels():
 
 class VocabXentResult:
     """``loss`` (scalar; the sum for reduction "none"), ``loss_rows`` [N] and ``lse`` [N] in float32, ``hits`` and
-    ``count`` (rows with a label) as int64 scalars on the device."""
+    ``count`` (rows with a label) as int64 scalars on the device.  ``rows`` [4, N] holds what a row leaves: its loss, the
+    logarithm of its sum of exponentials, its largest logit, and the sum of exponentials relative to that."""
 
-    __slots__ = ("loss", "loss_rows", "lse", "counts", "reduction", "ignore_index")
+    __slots__ = ("loss", "rows", "counts", "reduction", "ignore_index")
 
-    def __init__(self, loss, loss_rows, lse, counts, reduction, ignore_index):
-        self.loss, self.loss_rows, self.lse, self.counts = loss, loss_rows, lse, counts
+    def __init__(self, loss, rows, counts, reduction, ignore_index):
+        self.loss, self.rows, self.counts = loss, rows, counts
         self.reduction, self.ignore_index = reduction, ignore_index
+
+    @property
+    def loss_rows(self) -> torch.Tensor:
+        return self.rows[0]
+
+    @property
+    def lse(self) -> torch.Tensor:
+        return self.rows[1]
 
     @property
     def hits(self) -> torch.Tensor:
@@ -96,14 +105,16 @@ def _rows(t):
     return t, ld
 
 
-def _build(features, weight, labels, bias, lse, counts, ignore_index, mean):
+def _build(features, weight, labels, bias, rows, counts, ignore_index, mean):
     code, wcode = _check(features, weight, labels, bias)
     x, ldx = _rows(features)
     w, ldw = _rows(weight)
     b = None if bias is None else bias.detach().float().contiguous()
     labels = labels.contiguous()
     a = _Args()
-    a.X, a.W, a.labels, a.lse, a.counts = x.data_ptr(), w.data_ptr(), labels.data_ptr(), lse.data_ptr(), counts.data_ptr()
+    a.X, a.W, a.labels, a.counts = x.data_ptr(), w.data_ptr(), labels.data_ptr(), counts.data_ptr()
+    at, step = rows.data_ptr(), 4 * rows.shape[1]
+    a.loss_rows, a.lse, a.top, a.total = at, at + step, at + 2 * step, at + 3 * step
     a.bias = _lib.ptr(b)
     a.ignore, a.ldx, a.ldw, a.V, a.N, a.D = ignore_index, ldx, ldw, w.shape[0], x.shape[0], x.shape[1]
     a.dtype, a.w_dtype, a.mean = code, wcode, int(mean)
@@ -128,20 +139,20 @@ def vocab_xent_fwd(features: torch.Tensor, weight: torch.Tensor, labels: torch.T
     n, dev = features.shape[0], features.device
     if n == 0:
         _check(features, weight, labels, bias)
-        none = features.new_zeros(0, dtype=torch.float32)
-        return VocabXentResult(features.new_zeros((), dtype=torch.float32), none, none, labels.new_zeros(2), reduction, ignore_index)
+        return VocabXentResult(features.new_zeros((), dtype=torch.float32), features.new_zeros((4, 0), dtype=torch.float32),
+                               labels.new_zeros(2), reduction, ignore_index)
     if not features.is_cuda:
         _check(features, weight, labels, bias)
         return VocabXentResult(*reference.vocab_xent(features, weight, labels, bias, ignore_index, reduction), reduction, ignore_index)
-    rows = features.new_empty((2, n), dtype=torch.float32)
+    rows = features.new_empty((4, n), dtype=torch.float32)
     loss = features.new_empty((), dtype=torch.float32)
     counts = features.new_empty(2, dtype=torch.int64)
-    a, keep = _build(features, weight, labels, bias, rows[1], counts, ignore_index, reduction == "mean")
-    a.loss_rows, a.loss = rows.data_ptr(), loss.data_ptr()
+    a, keep = _build(features, weight, labels, bias, rows, counts, ignore_index, reduction == "mean")
+    a.loss = loss.data_ptr()
     ws = _workspace(a, 0, dev)
     launch("vocab_xent_fwd", _kernels().dtf_vocab_xent_fwd, features, C.byref(a))
     del keep, ws
-    return VocabXentResult(loss, rows[0], rows[1], counts, reduction, ignore_index)
+    return VocabXentResult(loss, rows, counts, reduction, ignore_index)
 
 
 def vocab_xent_bwd(fwd: VocabXentResult, features: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
@@ -153,8 +164,8 @@ def vocab_xent_bwd(fwd: VocabXentResult, features: torch.Tensor, weight: torch.T
     per_row = fwd.reduction == "none"
     if dloss is not None and (dloss.dtype != torch.float32 or dloss.numel() != (n if per_row else 1)):
         raise ValueError("vocab_xent_bwd: dloss must be float32, a scalar or (reduction \"none\") one value a row")
-    same_device("vocab_xent_bwd", features, dloss, fwd.lse)
-    if fwd.lse.shape[0] != n:
+    same_device("vocab_xent_bwd", features, dloss, fwd.rows)
+    if fwd.rows.shape[1] != n:
         raise ValueError("vocab_xent_bwd: the forward result belongs to another batch")
     if n == 0:
         _check(features, weight, labels, bias)
@@ -164,7 +175,7 @@ def vocab_xent_bwd(fwd: VocabXentResult, features: torch.Tensor, weight: torch.T
         _check(features, weight, labels, bias)
         d = reference.vocab_xent_bwd(features, weight, labels, bias, fwd.lse, fwd.counts, fwd.ignore_index, fwd.reduction, dloss)
         return d[0] if want_x else None, d[1] if want_w else None, d[2] if want_b else None
-    a, keep = _build(features, weight, labels, bias, fwd.lse, fwd.counts, fwd.ignore_index, fwd.reduction == "mean")
+    a, keep = _build(features, weight, labels, bias, fwd.rows, fwd.counts, fwd.ignore_index, fwd.reduction == "mean")
     dx = torch.empty(features.shape, dtype=features.dtype, device=dev) if want_x else None
     dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
     db = torch.empty(weight.shape[0], dtype=torch.float32, device=dev) if want_b else None
@@ -183,17 +194,17 @@ class _VocabXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, weight, labels, bias, ignore_index, reduction):
         r = vocab_xent_fwd(features, weight, labels, bias, ignore_index, reduction)
-        ctx.save_for_backward(features, weight, labels, bias, r.lse, r.counts)
+        ctx.save_for_backward(features, weight, labels, bias, r.rows, r.counts)
         ctx.reduction, ctx.ignore_index = reduction, ignore_index
         hits = r.counts[0].clone()
         ctx.mark_non_differentiable(hits)
-        return (r.loss_rows if reduction == "none" else r.loss), hits
+        return (r.loss_rows.clone() if reduction == "none" else r.loss), hits       # what backward() reads stays its own
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _dhits):
-        features, weight, labels, bias, lse, counts = ctx.saved_tensors
-        fwd = VocabXentResult(None, None, lse, counts, ctx.reduction, ctx.ignore_index)
+        features, weight, labels, bias, rows, counts = ctx.saved_tensors
+        fwd = VocabXentResult(None, rows, counts, ctx.reduction, ctx.ignore_index)
         need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
         dx, dw, db = vocab_xent_bwd(fwd, features, weight, labels, bias, dloss, need)
         return dx, dw, None, db, None, None
