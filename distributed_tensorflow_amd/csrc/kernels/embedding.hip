@@ -6,11 +6,11 @@
 // The gradient is a segmented sum.  Tokens are sorted by id, stably, so a row's tokens stand in the order of their
 // positions; a row with tokens is then written by one workgroup: no atomics on floats (the same inputs give the same bits)
 // and no fp32 table in between.
-//   sort    LSD radix sort of (id, position) with digits of at most 9 bits (32 KB of counters): up to 16384 tokens in ONE
+//   sort    LSD radix sort of (id, position) with digits of at most 9 bits (32 KB of counters): up to 8192 tokens in ONE
 //           workgroup and launch, else count / scatter launches over blocks of 4096 tokens.  The sort keeps a few CUs busy;
 //           the other workgroups of its launches fill the table's gradient with zeros meanwhile (measured apart: 39 us of
-//           sorting 16384 tokens, 25 us of filling 50001 x 1024 bf16).
-//   chunks  The sorted list is cut into chunks of 32 tokens or more, one workgroup (or part of one) each, so that frequent
+//           sorting 16384 tokens in one workgroup, 25 us of filling 50001 x 1024 bf16).
+//   chunks  The sorted list is cut into chunks of 16 tokens or more, one workgroup (or part of one) each, so that frequent
 //           rows are shared: rows inside a chunk are summed in fp32, scaled, rounded once and stored; of a row that crosses
 //           the chunk's border (at most two do) the sum is kept as a part.
 //   join    The chunk in which a crossing row starts adds the row's parts in order and stores it.
@@ -22,7 +22,7 @@
 #include "token_ops.h"
 
 namespace {
-constexpr int kOne = 16384;                      // tokens that one workgroup sorts
+constexpr int kOne = 8192;                       // tokens that one workgroup sorts
 constexpr int kSortBlock = 1024, kSortWaves = kSortBlock / 64;
 constexpr int kKeys = 4096;                      // tokens a workgroup of the multi-launch sort
 constexpr int kMaxBits = 9;
@@ -116,6 +116,7 @@ __device__ __forceinline__ void rank_in_wave(const int (&key)[ROUNDS], int live,
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
+    if (64 * r >= live) break;                   // the same for the whole wave
     const bool active = 64 * r + lane < live;
     const int digit = (key[r] >> shift) & ((1 << bits) - 1);
     const unsigned long long same = same_digit(digit, bits, active);
@@ -391,7 +392,7 @@ EmbPlan plan(int64_t n, int64_t V, int D) {
   p.passes = (total + kMaxBits - 1) / kMaxBits;
   p.bits = (total + p.passes - 1) / p.passes;
   p.blocks = (int)((n + kKeys - 1) / kKeys);
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(32, n / 4096), 1024);
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(16, n / 2048), 1024);
   p.chunks = (int)((n + p.chunk - 1) / p.chunk);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
