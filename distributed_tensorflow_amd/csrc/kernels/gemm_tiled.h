@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void gemm_tiled_kernel(Args p) {
   if constexpr (EPI >= EPI_CUSTOM) {       // the barrier that ends the main loop leaves the staging buffers free
     static_assert(TI == 4 && TJ == 4, "one 16 KB piece of the staging buffers for each wave's 64x64 block");
     unsigned char* const wl = (wave < 2 ? lds_a[wave] : lds_b[wave - 2]);
-    p.template epilogue<EPI & ~EPI_PLANES, (EPI >= EPI_PLANES)>(acc, wl, m0 + wm * 64, n0 + wn * 64, lane);
+    p.template epilogue<EPI & ~EPI_PLANES, (EPI >= EPI_PLANES || sizeof(T) == 4)>(acc, wl, m0 + wm * 64, n0 + wn * 64, lane);
     return;
   }
   // ---------------- epilogue: acc[i][j][r] = C[m0 + wm*16*TI + 16i + 4g + r][n0 + wn*16*TJ + 16j + fr]

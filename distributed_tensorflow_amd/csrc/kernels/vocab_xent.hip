@@ -23,7 +23,8 @@
 // a sixteenth.  (Elements below 2^-110 lose their last planes: 10^-33 beside sums of order one.)
 //
 // Kernels: the 8-wave 256x256 GEMM (gemm_pingpong.h) where its blocks fill the chip, the 4-wave 128x128 one (gemm_tiled.h)
-// otherwise; logits of few rows or columns by a kernel that shares K between the waves (fp32: fp32 matrix instructions).
+// otherwise; logits of few rows or columns by a kernel that shares K between the waves; the products of few rows
+// by kernels that read W and write dW once, with fp32 matrix instructions, as have fp32 logits of under 256 rows.
 // bf16 widths that are no multiple of 16 bytes, unaligned or strided operands go through zero-padded copies, piece by piece.
 #include <hip/hip_runtime.h>
 
@@ -35,7 +36,7 @@
 #include "token_ops.h"
 
 namespace {
-enum { VX_LSE = EPI_CUSTOM, VX_DZ = EPI_CUSTOM + 1, VX_SUM = EPI_CUSTOM + 2 };
+enum { VX_LSE = EPI_CUSTOM, VX_DZ = EPI_CUSTOM + 1, VX_SUM = EPI_CUSTOM + 2, VX_DZ32 = EPI_CUSTOM + 3 };   // VX_DZ32: dz in fp32
 constexpr int kStrip = 64;                       // columns a wave reduces in the forward pass
 constexpr int kLseSplits = 16;                   // waves of the join that share a row's strips
 
@@ -89,7 +90,7 @@ struct VxGemm : DtfGemmArgs {
   float2* target;                                // [M]: the label's logit, whether an earlier column of its strip reaches it
   int v0;                                        // vocabulary index of column 0
   // VX_DZ (C = dz [M, ldc], Ct = dz^T [N, ldct]; both leading dimensions are the padded widths, padding is zeroed; of fp32
-  // operands only C, in fp32)
+  // operands, and as VX_DZ32, only C, in fp32)
   const VxRow* rows;                             // padded to the block height
   unsigned a_plane, b_plane;                     // bytes between the planes of the operands (EPI_PLANES)
   float* db_part;                                // [wave rows][N], optional
@@ -126,6 +127,7 @@ struct VxGemm : DtfGemmArgs {
       store_sum<RI>(acc, wl, crow, ccol, lane);
       return;
     }
+    constexpr bool kF32Out = F32 || EPI == VX_DZ32;
     const float NEG_INF = -__builtin_huge_valf();
     if (bias) {
 #pragma unroll
@@ -203,7 +205,7 @@ struct VxGemm : DtfGemmArgs {
 #pragma unroll
           for (int cj = 0; cj < 4; ++cj) {
             const float d = acc[ri][cj][r] - row.top;
-            acc[ri][cj][r] = row.g == 0.f ? 0.f : (F32 ? exp_exact(d) : __expf(d)) * row.scaled;
+            acc[ri][cj][r] = row.g == 0.f ? 0.f : (kF32Out ? exp_exact(d) : __expf(d)) * row.scaled;
           }
         }
       }
@@ -234,7 +236,7 @@ struct VxGemm : DtfGemmArgs {
           if (g == 0 && col < N) db_part[(size_t)(crow / (16 * RI)) * N + col] = v;
         }
       }
-      if constexpr (F32) {
+      if constexpr (kF32Out) {
         float* const c = static_cast<float*>(C);
 #pragma unroll
         for (int ri = 0; ri < RI; ++ri)
@@ -395,6 +397,117 @@ __global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[0][j][r] = ((acc[0][j][r] + s_acc[0][4 * j + r][lane]) + s_acc[1][4 * j + r][lane]) + s_acc[2][4 * j + r][lane];
   p.template epilogue<EPI, sizeof(T) == 4>(acc, s_out, m0, n0, lane);
+}
+
+// The products of few rows (use_small), straight from X, W and the fp32 dz, with fp32 matrix instructions: the time goes
+// into reading W and writing dW once, so no transposed copies and no planes are made.  A lane's 16-byte piece of a row of W
+// (or X) is the operand of VEC instructions at once: instruction q takes column c0 + VEC fr + q.
+
+// dX: workgroup (column tile, 16 rows, range of the vocabulary); the waves take 16 vocabulary rows each in turn.
+// ROUND: fp32 weights under bf16 activations, rounded as the logits' copy of them was.
+template <typename T, bool ROUND>
+__global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restrict__ dz, long lddz, const T* __restrict__ w, long ldw, float* __restrict__ out,
+                                                          int M, int D, long n, int per, int ldo) {
+  typedef TkPiece<T, false> P;
+  constexpr int VEC = P::VEC;
+  __shared__ float s_acc[3][4 * VEC][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
+  const int c = (int)blockIdx.x * 16 * VEC + VEC * fr, m0 = blockIdx.y * 16;
+  const long lo = (long)blockIdx.z * per, hi = min(n, lo + per);
+  f32x4 acc[VEC];
+#pragma unroll
+  for (int q = 0; q < VEC; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float* const arow = dz + (long)(m0 + fr < M ? m0 + fr : 0) * lddz;
+  for (long v = lo + 16 * wave; v < hi; v += 128) {
+    f32x4 a[2];
+    tk_u32x4 b[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const long at = v + 64 * u + 4 * g;        // dz is zero from n to its padded width, a multiple of 64 columns
+      a[u] = v + 64 * u < hi && m0 + fr < M ? *reinterpret_cast<const f32x4*>(arow + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[u][j] = at + j < hi && c < D ? P::load(w + (at + j) * ldw, c, D) : tk_u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float wv[VEC];
+        P::unpack(b[u][j], wv);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          if (ROUND) wv[q] = tk_bf2f(tk_f2bf(wv[q]));
+          acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][j], wv[q], acc[q], 0, 0, 0);
+        }
+      }
+  }
+  if (wave) {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_acc[wave - 1][4 * q + r][lane] = acc[q][r];
+  }
+  __syncthreads();
+  if (wave || c >= ldo) return;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = m0 + 4 * g + r;
+    if (row >= M) continue;
+    float* const o = out + ((size_t)blockIdx.z * M + row) * ldo + c;
+#pragma unroll
+    for (int q = 0; q < VEC; q += 4) {
+      f32x4 t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        t[e] = ((acc[q + e][r] + s_acc[0][4 * (q + e) + r][lane]) + s_acc[1][4 * (q + e) + r][lane]) + s_acc[2][4 * (q + e) + r][lane];
+      if (c + q < ldo) *reinterpret_cast<f32x4*>(o + q) = t;
+    }
+  }
+}
+
+// dW: a wave owns 16 vocabulary rows and 16 VEC columns.
+template <typename TX, typename TO>
+__global__ __launch_bounds__(256) void vx_small_dw_kernel(const float* __restrict__ dz, long lddz, const TX* __restrict__ x, long ldx, TO* __restrict__ out,
+                                                          int M, int D, long n, const float* __restrict__ scale) {
+  typedef TkPiece<TX, false> P;
+  constexpr int VEC = P::VEC, OUT = 16 / sizeof(TO);
+  const int lane = threadIdx.x & 63, fr = lane & 15, g = lane >> 4;
+  const int tiles = (D + 16 * VEC - 1) / (16 * VEC);
+  const long v0 = (long)(blockIdx.x / tiles) * 64 + 16 * (threadIdx.x >> 6);
+  const int c = (int)(blockIdx.x % tiles) * 16 * VEC + VEC * fr;
+  f32x4 acc[VEC];
+#pragma unroll
+  for (int q = 0; q < VEC; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < M; k += 16) {
+    float a[4];
+    tk_u32x4 b[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int row = k + 4 * u + g;
+      a[u] = row < M && v0 + fr < n ? dz[(long)row * lddz + v0 + fr] : 0.f;
+      b[u] = row < M && c < D ? P::load(x + (long)row * ldx, c, D) : tk_u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float xv[VEC];
+      P::unpack(b[u], xv);
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u], xv[q], acc[q], 0, 0, 0);
+    }
+  }
+  const float f = *scale;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const long v = v0 + 4 * g + r;
+    if (v >= n) continue;
+#pragma unroll
+    for (int q = 0; q < VEC; q += OUT) {
+      float t[OUT];
+#pragma unroll
+      for (int e = 0; e < OUT; ++e) t[e] = acc[q + e][r] * f;
+      if (c + q < D) TkPiece<TO, false>::store(out + v * D, c + q, D, t);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------- streaming helpers
@@ -636,11 +749,28 @@ bool use_pp(int planes, long m, long n, long k, int splits) {
   return m >= 256 && n >= 256 && k / splits >= 256 && blocks >= (deep >= 2048 ? 112 : 192);
 }
 
-// 128x128 blocks would leave most CUs idle, or their rows mostly empty
-bool use_skinny(long m, long n) { return m <= 16 || ((m + 127) / 128) * ((n + 127) / 128) < 128; }
+// Up to so many rows the products read W and X as they are (vx_small_dx_kernel, vx_small_dw_kernel).  Backward pass at
+// 131072 x 4096, this way / through transposed copies: bf16 32 rows 1.04 / 1.21 ms, 64 rows 1.65 / 1.22; fp32 64 rows 3.4 / 5.3.
+bool use_small(int dtype, long m) { return m <= (dtype == TK_BF16 ? 32 : 64); }
+
+// Logits by the kernel that shares K between the waves: where 128x128 blocks would leave most CUs idle or, with few rows, be
+// mostly empty (bf16: as long as W is small; a large one streams faster through the 128x128 blocks: 131072 x 4096, one row,
+// 203 against 227 us); fp32 with few rows always (its 128x128 blocks compute 128 rows at a
+// sixteenth of the bf16 rate: 1.1 ms for 131072 x 4096, which three tiles of 16 rows reach).
+bool use_skinny(int dtype, long m, long n) {
+  const long blocks = ((m + 127) / 128) * ((n + 127) / 128);
+  return blocks < 128 || (dtype == TK_F32 ? m <= 48 : m <= 16 && blocks < 512);
+}
+
+// fp32 logits from planes: they cost 10 bytes of traffic for every element of W, which pays from about 256 rows on (131072 x
+// 4096, 64 rows: 2.5 ms through planes).
+bool use_planes(int dtype, long m, bool skinny) { return dtype == TK_F32 && !skinny && m >= 256; }
+
+// fp32 operands as they are
+bool direct_f32(const VxGemm& a) { return a.dtype == TK_F32 && a.a_plane == 0; }
 
 // Rows of a wave's block in the logits' epilogue
-int wave_rows(const VxGemm& a, bool skinny) { return skinny ? 16 : use_pp(a.a_plane ? 3 : 1, a.M, a.N, a.K, 1) ? 128 : 64; }
+int wave_rows(const VxGemm& a, bool skinny) { return skinny ? 16 : direct_f32(a) ? 64 : use_pp(a.a_plane ? 3 : 1, a.M, a.N, a.K, 1) ? 128 : 64; }
 
 template <int EPI>
 void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
@@ -657,11 +787,18 @@ void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
 }
 
 template <int EPI>
-void launch_logits(const VxGemm& a, bool skinny, hipStream_t s) {
-  if (!skinny) return launch_gemm<EPI>(a, 1, s);
+void launch_skinny(const VxGemm& a, hipStream_t s) {
   const dim3 g((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64)));
   if (a.dtype == TK_BF16) hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI>), g, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI>), g, dim3(256), 0, s, a);
+}
+
+template <int EPI>
+void launch_logits(const VxGemm& a, bool skinny, hipStream_t s) {
+  if (skinny) launch_skinny<EPI>(a, s);
+  else if (direct_f32(a))
+    hipLaunchKernelGGL((gemm_tiled_kernel<unsigned int, EPI, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
+  else launch_gemm<EPI>(a, 1, s);
 }
 
 // planes: 3 bf16 planes an operand, each dense; 1: the operands are of type dtype
@@ -699,7 +836,7 @@ struct VxPlan {
   long Dp, Np, Vp, pieces, strips, blocks, ldd, ldn, ldv;
   int K;                                         // of the logits: padded only where both operands are
   int planes;                                    // of every operand of the large products
-  bool skinny, pack_x, pack_w, direct_dx, direct_dw;
+  bool skinny, direct, small, pack_x, pack_w, direct_dx, direct_dw;       // direct: the logits read X and W (or padded copies) as they are
   int sx, sw;                                    // splits of the two products
   size_t x, w, part, target, blk, rows, xt, wt, dz32, dz, dzt, dx32, dw32, db, total;
 };
@@ -728,14 +865,15 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.Vp = p.pieces == 1 ? a.V : std::min(vp, up((a.V + p.pieces - 1) / p.pieces, 256));
   p.pieces = (a.V + p.Vp - 1) / p.Vp;
   p.ldv = up(p.Vp, 64);
-  p.skinny = use_skinny(a.N, p.Vp);
-  // copies: bf16 where the operand's rows are no whole aligned 16-byte pieces; fp32 the same for the skinny kernel, planes
-  // for the others
+  p.skinny = use_skinny(a.dtype, a.N, p.Vp);
+  p.direct = !use_planes(a.dtype, a.N, p.skinny);
+  p.small = use_small(a.dtype, a.N);
+  // copies where the operand's rows are no whole aligned 16-byte pieces, or planes
   const bool odd_x = a.D % per16 || a.ldx % per16 || !dtf_aligned16(a.X), odd_w = a.D % per16 || a.ldw % per16 || !dtf_aligned16(a.W);
-  p.K = p.skinny && a.D % per16 == 0 ? a.D : (int)p.Dp;
-  p.pack_x = p.planes == 3 && !p.skinny ? true : odd_x;
-  p.pack_w = p.planes == 3 && !p.skinny ? true : odd_w || a.w_dtype != a.dtype;
-  const size_t copy = p.planes == 3 && !p.skinny ? 6 : es;
+  p.K = p.direct && a.D % per16 == 0 ? a.D : (int)p.Dp;
+  p.pack_x = p.direct ? odd_x : true;
+  p.pack_w = p.direct ? odd_w || a.w_dtype != a.dtype : true;
+  const size_t copy = p.direct ? es : 6;
   size_t at = 0;
   if (p.pack_x) p.x = take(at, (size_t)a.N * p.ldd * copy);
   if (p.pack_w) p.w = take(at, (size_t)p.Vp * p.ldd * copy);
@@ -748,20 +886,28 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   } else {
     const long Vpp = up(p.Vp, 8);
     p.rows = take(at, (size_t)up(a.N, 256) * sizeof(VxRow) + 16);     // and the common factor behind them
-    p.xt = take(at, (size_t)p.Dp * p.ldn * col);
-    p.wt = take(at, (size_t)p.Dp * p.ldv * col);
-    if (p.planes == 3) p.dz32 = take(at, (size_t)a.N * p.ldv * 4);
-    p.dz = take(at, (size_t)a.N * p.ldv * col);
-    p.dzt = take(at, (size_t)p.Vp * p.ldn * col);
-    p.sx = splits_for(p.planes, a.N, p.Dp, Vpp);
-    p.sw = splits_for(p.planes, p.Vp, p.Dp, p.Np);
-    p.sx = (int)((Vpp + kper_for(Vpp, p.sx) - 1) / kper_for(Vpp, p.sx));
-    p.sw = (int)((p.Np + kper_for(p.Np, p.sw) - 1) / kper_for(p.Np, p.sw));
-    // straight into the result where one product (or the last piece's) holds the whole sum at a 16-byte row width
-    p.direct_dx = p.sx == 1 && p.Dp == a.D && dtf_aligned16(a.dX);
-    p.direct_dw = p.sw == 1 && p.Dp == a.D && dtf_aligned16(a.dW);
-    if (!p.direct_dx || (a.dtype == TK_BF16 && p.pieces > 1)) p.dx32 = take(at, (size_t)p.sx * a.N * p.Dp * 4);
-    if (!p.direct_dw) p.dw32 = take(at, (size_t)p.sw * p.Vp * p.Dp * 4);
+    if (p.small) {
+      p.dz32 = take(at, (size_t)a.N * p.ldv * 4);
+      // column tiles x row tiles x ranges of the vocabulary: about 1024 workgroups, ranges of 256 or more
+      const long tiles = ((a.D + 16 * (a.w_dtype == TK_BF16 ? 8 : 4) - 1) / (16 * (a.w_dtype == TK_BF16 ? 8 : 4))) * ((a.N + 15) / 16);
+      p.sx = (int)std::max<long>(1, std::min<long>({1024 / tiles, p.Vp / 256, 256}));
+      p.dx32 = take(at, (size_t)p.pieces * p.sx * a.N * p.Dp * 4);
+    } else {
+      p.xt = take(at, (size_t)p.Dp * p.ldn * col);
+      p.wt = take(at, (size_t)p.Dp * p.ldv * col);
+      if (p.planes == 3) p.dz32 = take(at, (size_t)a.N * p.ldv * 4);
+      p.dz = take(at, (size_t)a.N * p.ldv * col);
+      p.dzt = take(at, (size_t)p.Vp * p.ldn * col);
+      p.sx = splits_for(p.planes, a.N, p.Dp, Vpp);
+      p.sw = splits_for(p.planes, p.Vp, p.Dp, p.Np);
+      p.sx = (int)((Vpp + kper_for(Vpp, p.sx) - 1) / kper_for(Vpp, p.sx));
+      p.sw = (int)((p.Np + kper_for(p.Np, p.sw) - 1) / kper_for(p.Np, p.sw));
+      // straight into the result where one product (or the last piece's) holds the whole sum at a 16-byte row width
+      p.direct_dx = p.sx == 1 && p.Dp == a.D && dtf_aligned16(a.dX);
+      p.direct_dw = p.sw == 1 && p.Dp == a.D && dtf_aligned16(a.dW);
+      if (!p.direct_dx || (a.dtype == TK_BF16 && p.pieces > 1)) p.dx32 = take(at, (size_t)p.sx * a.N * p.Dp * 4);
+      if (!p.direct_dw) p.dw32 = take(at, (size_t)p.sw * p.Vp * p.Dp * 4);
+    }
     if (a.dbias) p.db = take(at, (size_t)(a.N / 16 + 4) * p.Vp * 4);       // one row of partial sums for every 16 rows at most
   }
   p.total = at;
@@ -805,18 +951,39 @@ void planes(const void* src, void* dst, void* dst_t, long M, long N, long lds_, 
 struct Operand { const void* p; long ld; };
 Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int from, long rows, long ld, bool copy, void* dst, void* to_t, long ldt, hipStream_t s) {
   Operand o = {src, ld};
-  if (p.planes == 3) {
-    if (!p.skinny || to_t) planes(src, p.skinny ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), s);
-    if (p.skinny && copy) pack(src, from, dst, TK_F32, rows, a.D, ld, p.ldd, s);
-    if (!p.skinny || copy) o = {dst, p.ldd};
-  } else {
-    if (copy) {
-      pack(src, from, dst, TK_BF16, rows, a.D, ld, p.ldd, s);
-      o = {dst, p.ldd};
-    }
-    if (to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, s);
-  }
+  if (!p.direct || (p.planes == 3 && to_t)) planes(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), s);
+  if (p.direct && copy) pack(src, from, dst, a.dtype, rows, a.D, ld, p.ldd, s);
+  if (copy) o = {dst, p.ldd};
+  if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, s);
   return o;
+}
+
+// dz in fp32 for the kernels of few rows
+void launch_small_dz(const VxGemm& a, bool skinny, hipStream_t s) {
+  if (a.dtype == TK_F32) launch_logits<VX_DZ>(a, skinny, s);           // fp32 operands leave fp32
+  else if (skinny) launch_skinny<VX_DZ32>(a, s);
+  else hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, VX_DZ32, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
+}
+
+void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
+  const int vec = a.w_dtype == TK_BF16 ? 8 : 4;
+  const int per = (int)up((p.Vp + p.sx - 1) / p.sx, 64);
+  const dim3 g((unsigned)dtf_cdiv(a.D, 16 * vec), (unsigned)dtf_cdiv(a.N, 16), (unsigned)p.sx);
+  auto go = [&](auto kernel, auto* wt) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, dz, lddz, wt, (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp); };
+  if (a.w_dtype == TK_BF16) go(vx_small_dx_kernel<unsigned short, false>, static_cast<const unsigned short*>(w));
+  else if (a.dtype == TK_BF16) go(vx_small_dx_kernel<float, true>, static_cast<const float*>(w));
+  else go(vx_small_dx_kernel<float, false>, static_cast<const float*>(w));
+}
+
+template <typename TX, typename TO>
+void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const float* scale, hipStream_t s) {
+  const long blocks = ((n + 63) / 64) * dtf_cdiv(a.D, 16 * (16 / (int)sizeof(TX)));
+  hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx, static_cast<TO*>(out), a.N, a.D, n, scale);
+}
+void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const float* scale, hipStream_t s) {
+  if (a.dtype == TK_F32) small_dw_as<float, float>(a, dz, lddz, n, out, scale, s);
+  else if (a.w_dtype == TK_F32) small_dw_as<unsigned short, float>(a, dz, lddz, n, out, scale, s);
+  else small_dw_as<unsigned short, unsigned short>(a, dz, lddz, n, out, scale, s);
 }
 
 int check(const DtfVocabXentArgs* a) {
@@ -845,7 +1012,7 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
   const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, nullptr, 0, s);
-  const int large = p.skinny ? 1 : p.planes;     // planes of the logits' operands
+  const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0);
     const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w, nullptr, 0, s);
@@ -873,8 +1040,8 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW ? ws + p.xt : nullptr, p.ldn, s);
-  const int large = p.skinny ? 1 : p.planes;     // planes of the logits' operands
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW && !p.small ? ws + p.xt : nullptr, p.ldn, s);
+  const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   VxRow* const rows = reinterpret_cast<VxRow*>(ws + p.rows);
   const int Mp = (int)up(a.N, 256);
   float* const scale = reinterpret_cast<float*>(rows + Mp);
@@ -884,20 +1051,27 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0), np = up(n, 8), ldv = up(n, 64);
     const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w,
-                              a.dX ? ws + p.wt : nullptr, ldv, s);
+                              a.dX && !p.small ? ws + p.wt : nullptr, ldv, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.rows = rows;
     g.v0 = (int)v0;
-    g.C = ws + (p.planes == 3 ? p.dz32 : p.dz);
+    g.C = ws + (p.planes == 3 || p.small ? p.dz32 : p.dz);
     g.ldc = (int)ldv;
     g.Ct = ws + p.dzt;
     g.ldct = (int)p.ldn;
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
-    launch_logits<VX_DZ>(g, p.skinny, s);
-    if (p.planes == 3) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, s);
+    if (p.small) launch_small_dz(g, p.skinny, s);
+    else launch_logits<VX_DZ>(g, p.skinny, s);
+    if (p.planes == 3 && !p.small) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, s);
     if (a.dbias)
       hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
+    if (p.small) {
+      const float* const dz = reinterpret_cast<const float*>(ws + p.dz32);
+      if (a.dX) small_dx(a, p, dz, ldv, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), n, dx32 + (size_t)(v0 / p.Vp) * p.sx * a.N * p.Dp, s);
+      if (a.dW) small_dw(a, dz, ldv, n, static_cast<char*>(a.dW) + v0 * a.D * (a.w_dtype == TK_BF16 ? 2 : 4), scale, s);
+      continue;
+    }
     if (a.dX) {
       VxGemm d = operands(ws + p.dz, ws + p.wt, TK_BF16, p.planes, a.N, (int)p.Dp, (int)np, ldv, ldv);
       const long kper = kper_for(up(p.Vp, 8), p.sx);
@@ -928,6 +1102,6 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
       if (!p.direct_dw) finish(dw32, p.sw, n, a.D, (int)p.Dp, out, a.D, a.w_dtype, scale, s);
     }
   }
-  if (a.dX && !p.direct_dx) finish(dx32, p.sx, a.N, a.D, (int)p.Dp, a.dX, a.D, a.dtype, scale, s);
+  if (a.dX && !p.direct_dx) finish(dx32, p.small ? (int)p.pieces * p.sx : p.sx, a.N, a.D, (int)p.Dp, a.dX, a.D, a.dtype, scale, s);
   return dtf_check_launch();
 }

@@ -94,7 +94,9 @@ def check(n, v, d, dtype, dev, wdtype=None, bias=True, reduction="mean", dloss=N
 
 
 SIZES = [(1, 1, 1), (1, 2, 8), (1, 1000, 64), (2, 63, 16), (3, 64, 24), (5, 65, 40), (7, 129, 100), (17, 257, 7), (100, 1000, 256),
-         (127, 10, 33), (128, 128, 128), (129, 300, 264), (300, 77, 72), (260, 515, 20)]
+         (127, 10, 33), (128, 128, 128), (129, 300, 264), (300, 77, 72), (260, 515, 20),
+         (16, 16500, 24), (17, 16500, 40), (32, 8200, 33), (33, 8200, 33), (48, 16500, 40), (49, 16500, 40), (64, 16500, 130), (65, 16500, 130),
+         (255, 9001, 48), (256, 9001, 48)]
 
 
 @pytest.mark.parametrize("dev", devices())
@@ -150,6 +152,7 @@ def test_reductions_and_upstream_gradients(reduction, dev):
 @pytest.mark.parametrize("dev", devices())
 def test_float32_weight_under_bfloat16_features(dev):
     check(90, 333, 72, torch.bfloat16, dev, wdtype=torch.float32)
+    check(40, 333, 71, torch.bfloat16, dev, wdtype=torch.float32)
 
 
 @pytest.mark.parametrize("dev", devices())
@@ -230,11 +233,12 @@ def test_labels_outside_the_vocabulary_are_nan_on_the_gpu():
 
 @pytest.mark.parametrize("dev", devices())
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_strides_alignment_and_label_views(dtype, dev):
-    x, w, lab, b = (t.to(dev) for t in draw(50, 150, 64, dtype))
+@pytest.mark.parametrize("n", [50, 90])
+def test_strides_alignment_and_label_views(n, dtype, dev):
+    x, w, lab, b = (t.to(dev) for t in draw(n, 150, 64, dtype))
     base = vx.vocab_xent_fwd(x, w, lab, b)
     grads = vx.vocab_xent_bwd(base, x, w, lab, b)
-    wide_x, wide_w = torch.zeros(50, 131, device=dev, dtype=dtype), torch.zeros(150, 80, device=dev, dtype=dtype)
+    wide_x, wide_w = torch.zeros(n, 131, device=dev, dtype=dtype), torch.zeros(150, 80, device=dev, dtype=dtype)
     wide_x[:, 3:67], wide_w[:, 8:72] = x, w
     two = torch.stack([lab, lab], 1)
     for xv, wv, lv in ((wide_x[:, 3:67], wide_w[:, 8:72], two[:, 0]), (x.t().contiguous().t(), w.t().contiguous().t(), lab)):
