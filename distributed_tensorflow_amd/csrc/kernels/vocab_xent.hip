@@ -14,7 +14,9 @@
 // A factor that all rows share (1 / count, the gradient of a scalar loss) multiplies the sums, not dz: the label's element
 // of dz is near -1 for every row that is not learned yet, and -1 is exact in bf16 where -1/count is off by up to 2^-8 in
 // the same direction in every row.
-// Bound by the matrix cores.  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
+// Bound by the matrix cores, which the products keep 74-86 % busy: 8192 x 131072 x 4096 bf16 takes 25.1 ms forward and
+// backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of the
+// logits' launches are a third of their time.  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
 // type (bf16: half a step 2^-8 of each element, the same rounding that any bf16 product of dz has).
 //
 // fp32 operands are cut into three bf16 planes, x = x0 + x1 + x2 up to 2^-26 |x| (each plane takes eight more bits), and a
@@ -468,7 +470,7 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
 // dW: a wave owns 16 vocabulary rows and 16 VEC columns.
 template <typename TX, typename TO>
 __global__ __launch_bounds__(256) void vx_small_dw_kernel(const float* __restrict__ dz, long lddz, const TX* __restrict__ x, long ldx, TO* __restrict__ out,
-                                                          int M, int D, long n, const float* __restrict__ scale) {
+                                                          int M, int D, long n, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
   typedef TkPiece<TX, false> P;
   constexpr int VEC = P::VEC, OUT = 16 / sizeof(TO);
   const int lane = threadIdx.x & 63, fr = lane & 15, g = lane >> 4;
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(256) void vx_small_dw_kernel(const float* __restric
     for (int u = 0; u < 4; ++u) {
       const int row = k + 4 * u + g;
       a[u] = row < M && v0 + fr < n ? dz[(long)row * lddz + v0 + fr] : 0.f;
-      b[u] = row < M && c < D ? P::load(x + (long)row * ldx, c, D) : tk_u32x4{0u, 0u, 0u, 0u};
+      b[u] = row < M && c < D && rows[row].g != 0.f ? P::load(x + (long)row * ldx, c, D) : tk_u32x4{0u, 0u, 0u, 0u};       // (see vx_transpose_kernel)
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -520,15 +522,17 @@ __global__ __launch_bounds__(256) void vx_pack_kernel(const TS* __restrict__ src
   tk_put(dst + i, c < cols ? tk_get(src + row * lds_ + c) : 0.f);
 }
 
-// dst[c, r] = src[r, c] for r < M, c < N; zeros for r in [M, ldt).  64 x 64 tiles through LDS.
-__global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short* __restrict__ src, unsigned short* __restrict__ dst, int M, int N, long lds_, int ldt) {
+// dst[c, r] = src[r, c] for r < M, c < N; zeros for r in [M, ldt) and, of X (rows given), for rows without a gradient: in dW
+// they meet dz = 0, and a padding row that holds NaN or infinities must not make a sum of it.  64 x 64 tiles through LDS.
+__global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short* __restrict__ src, unsigned short* __restrict__ dst, int M, int N, long lds_, int ldt,
+                                                           const VxRow* __restrict__ rows) {
   __shared__ unsigned short tile[64][72];
   const int across = (N + 63) >> 6, c0 = (int)(blockIdx.x % across) * 64, r0 = (int)(blockIdx.x / across) * 64;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int id = threadIdx.x + 256 * i, rr = id >> 3, ch = id & 7;
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (r0 + rr < M && c0 + ch * 8 < N) v = *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + rr) * lds_ + c0 + ch * 8);
+    if (r0 + rr < M && c0 + ch * 8 < N && !(rows && rows[r0 + rr].g == 0.f)) v = *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + rr) * lds_ + c0 + ch * 8);
     *reinterpret_cast<u32x4*>(&tile[rr][ch * 8]) = v;
   }
   __syncthreads();
@@ -544,9 +548,9 @@ __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short*
 }
 
 // The three bf16 planes of an fp32 matrix [M, N] (any stride and alignment), straight [3][M, Np] and / or transposed
-// [3][Nt, Mp], zeros in the padding.
+// [3][Nt, Mp], zeros in the padding; in the transposed one also for rows without a gradient (see vx_transpose_kernel).
 __global__ __launch_bounds__(256) void vx_planes_kernel(const float* __restrict__ src, unsigned short* __restrict__ dst, unsigned short* __restrict__ dst_t,
-                                                        int M, int N, long lds_, int Np, int Nt, int Mp) {
+                                                        int M, int N, long lds_, int Np, int Nt, int Mp, const VxRow* __restrict__ rows) {
   __shared__ float tile[64][65];
   const int across = (Np + 63) >> 6, c0 = (int)(blockIdx.x % across) * 64, r0 = (int)(blockIdx.x / across) * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll
@@ -567,7 +571,10 @@ __global__ __launch_bounds__(256) void vx_planes_kernel(const float* __restrict_
       const int l = line + 32 * i, row = (turn ? c0 : r0) + l;
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = turn ? tile[ch * 8 + k][l] : tile[l][ch * 8 + k];
+      for (int k = 0; k < 8; ++k) {
+        v[k] = turn ? tile[ch * 8 + k][l] : tile[l][ch * 8 + k];
+        if (turn && rows && at + k < M && rows[at + k].g == 0.f) v[k] = 0.f;
+      }
       if (row < lines && at < ld) {
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
@@ -935,26 +942,27 @@ void pack(const void* src, int sdt, void* dst, int ddt, long rows, int cols, lon
   else pack_as<unsigned short, unsigned short>(src, dst, rows, cols, lds_, ldd, s);
 }
 
-void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, hipStream_t s) {
+void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, const VxRow* rows, hipStream_t s) {
   const dim3 g((unsigned)(((N + 63) / 64) * ((ldt + 63) / 64)));            // one index: there may be more than 65535 tile rows
-  hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt);
+  hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt, rows);
 }
 
-void planes(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, hipStream_t s) {
+void planes(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, const VxRow* rows, hipStream_t s) {
   const dim3 g((unsigned)(((Np + 63) / 64) * ((Mp + 63) / 64)));
   hipLaunchKernelGGL(vx_planes_kernel, g, dim3(256), 0, s, static_cast<const float*>(src), static_cast<unsigned short*>(dst), static_cast<unsigned short*>(dst_t),
-                     (int)M, (int)N, lds_, (int)Np, (int)Nt, (int)Mp);
+                     (int)M, (int)N, lds_, (int)Np, (int)Nt, (int)Mp, rows);
 }
 
 // One operand of the logits ([rows, D] of `from`, ld apart) as the kernel reads it, and transposed for a product (bf16: from
 // the aligned copy; to_t null: not needed).
 struct Operand { const void* p; long ld; };
-Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int from, long rows, long ld, bool copy, void* dst, void* to_t, long ldt, hipStream_t s) {
+Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int from, long rows, long ld, bool copy, void* dst, void* to_t, long ldt,
+                const VxRow* row_info, hipStream_t s) {
   Operand o = {src, ld};
-  if (!p.direct || (p.planes == 3 && to_t)) planes(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), s);
+  if (!p.direct || (p.planes == 3 && to_t)) planes(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), row_info, s);
   if (p.direct && copy) pack(src, from, dst, a.dtype, rows, a.D, ld, p.ldd, s);
   if (copy) o = {dst, p.ldd};
-  if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, s);
+  if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, row_info, s);
   return o;
 }
 
@@ -976,14 +984,14 @@ void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long 
 }
 
 template <typename TX, typename TO>
-void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const float* scale, hipStream_t s) {
+void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
   const long blocks = ((n + 63) / 64) * dtf_cdiv(a.D, 16 * (16 / (int)sizeof(TX)));
-  hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx, static_cast<TO*>(out), a.N, a.D, n, scale);
+  hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx, static_cast<TO*>(out), a.N, a.D, n, rows, scale);
 }
-void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const float* scale, hipStream_t s) {
-  if (a.dtype == TK_F32) small_dw_as<float, float>(a, dz, lddz, n, out, scale, s);
-  else if (a.w_dtype == TK_F32) small_dw_as<unsigned short, float>(a, dz, lddz, n, out, scale, s);
-  else small_dw_as<unsigned short, unsigned short>(a, dz, lddz, n, out, scale, s);
+void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
+  if (a.dtype == TK_F32) small_dw_as<float, float>(a, dz, lddz, n, out, rows, scale, s);
+  else if (a.w_dtype == TK_F32) small_dw_as<unsigned short, float>(a, dz, lddz, n, out, rows, scale, s);
+  else small_dw_as<unsigned short, unsigned short>(a, dz, lddz, n, out, rows, scale, s);
 }
 
 int check(const DtfVocabXentArgs* a) {
@@ -1011,11 +1019,11 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, nullptr, 0, s);
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, nullptr, 0, nullptr, s);
   const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0);
-    const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w, nullptr, 0, s);
+    const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w, nullptr, 0, nullptr, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.labels = a.labels;
@@ -1040,18 +1048,18 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW && !p.small ? ws + p.xt : nullptr, p.ldn, s);
-  const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   VxRow* const rows = reinterpret_cast<VxRow*>(ws + p.rows);
   const int Mp = (int)up(a.N, 256);
   float* const scale = reinterpret_cast<float*>(rows + Mp);
   hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.top, a.total, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, rows, scale);
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW && !p.small ? ws + p.xt : nullptr, p.ldn, rows, s);
+  const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   float* const dx32 = reinterpret_cast<float*>(ws + p.dx32);
   float* const dw32 = reinterpret_cast<float*>(ws + p.dw32);
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0), np = up(n, 8), ldv = up(n, 64);
     const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w,
-                              a.dX && !p.small ? ws + p.wt : nullptr, ldv, s);
+                              a.dX && !p.small ? ws + p.wt : nullptr, ldv, nullptr, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.rows = rows;
@@ -1063,13 +1071,13 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
     if (p.small) launch_small_dz(g, p.skinny, s);
     else launch_logits<VX_DZ>(g, p.skinny, s);
-    if (p.planes == 3 && !p.small) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, s);
+    if (p.planes == 3 && !p.small) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, nullptr, s);
     if (a.dbias)
       hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
     if (p.small) {
       const float* const dz = reinterpret_cast<const float*>(ws + p.dz32);
       if (a.dX) small_dx(a, p, dz, ldv, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), n, dx32 + (size_t)(v0 / p.Vp) * p.sx * a.N * p.Dp, s);
-      if (a.dW) small_dw(a, dz, ldv, n, static_cast<char*>(a.dW) + v0 * a.D * (a.w_dtype == TK_BF16 ? 2 : 4), scale, s);
+      if (a.dW) small_dw(a, dz, ldv, n, static_cast<char*>(a.dW) + v0 * a.D * (a.w_dtype == TK_BF16 ? 2 : 4), rows, scale, s);
       continue;
     }
     if (a.dX) {

@@ -231,7 +231,9 @@ def vocab_xent_bwd(features, weight, labels, bias, lse, counts, ignore_index=-10
     g = torch.where(valid, g.expand(x.shape[0]), torch.zeros((), device=x.device))
     dz = torch.exp(z - lse[:, None])
     dz.scatter_add_(1, lab[:, None], torch.full_like(lse, -1.0)[:, None])
-    dz = dz * g[:, None]
+    used = (g != 0)[:, None]                       # a row without a gradient may hold anything, also NaN
+    dz = torch.where(used, dz * g[:, None], torch.zeros((), device=x.device))
+    x = torch.where(used, x, torch.zeros((), device=x.device))
     db = None if bias is None else dz.sum(0).to(bias.dtype)
     return (dz @ w).to(features.dtype), (dz.t() @ x).to(weight.dtype), db
 

@@ -8,7 +8,8 @@ of about 1 GiB (or 16384 columns, whatever is more) backward, at any vocabulary 
 
 * types: float32 or bfloat16 features; a weight of the same type, or float32 under bfloat16 features (a bfloat16 copy is
   made piece by piece, its gradient is float32).  Logits, loss and statistics are float32.
-* ``labels``: int64 class indices.  A row whose label is ``ignore_index`` has loss 0, gives no gradient and does not count.
+* ``labels``: int64 class indices.  A row whose label is ``ignore_index`` has loss 0, gives no gradient and does not count,
+  whatever its features hold (also NaN).
   A label outside the vocabulary raises on the CPU; on the GPU, where raising would need a synchronisation, its row's
   loss (and with it the total) is NaN and the row gives no gradient.
 * ``reduction``: "mean" over the rows with a label (0 if there is none), "sum", or "none" (a loss per row).

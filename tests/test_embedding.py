@@ -81,6 +81,8 @@ def test_padding_index_and_id_types(idtype, dev):
     dy = torch.randn(900, 40)
     a = em.embedding_bwd(dy.to(dev), ids.to(dev), 50, 1.0, -50)
     assert not a[0].any()
+    dy[ids == 0] = float("nan")                      # what padding tokens bring does not matter
+    assert torch.equal(em.embedding_bwd(dy.to(dev), ids.to(dev), 50, 1.0, 0), a)
 
 
 @pytest.mark.parametrize("dev", devices())

@@ -211,6 +211,23 @@ def test_nan_stays_in_its_row(dev):
     assert torch.equal(r.loss_rows[others], clean.loss_rows[others]) and torch.isfinite(dx[others]).all()
 
 
+@pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v", [(20, 100), (60, 300), (100, 300), (300, 16400)])
+def test_padding_rows_may_hold_nan_and_infinity(n, v, dtype, dev):
+    """Every path of the backward pass: rows with the ignored label are as good as rows of zeros."""
+    x, w, lab, b = draw(n, v, 40, dtype)
+    lab[::3] = IGN
+    zero, junk = x.clone(), x.clone()
+    zero[::3] = 0
+    junk[0::6], junk[3::6] = float("nan"), float("inf")
+    r0, g0 = run(zero, w, lab, b, dev)
+    r1, g1 = run(junk, w, lab, b, dev)
+    assert torch.equal(r0.loss, r1.loss) and torch.equal(r0.loss_rows, r1.loss_rows) and torch.equal(r0.counts, r1.counts)
+    for a, c in zip(g0, g1):
+        assert torch.isfinite(c).all() and torch.equal(a, c)
+
+
 def test_labels_outside_the_vocabulary_raise_on_the_cpu():
     x, w, lab, b = draw(6, 20, 8, torch.float32)
     for bad in (20, -1, 1 << 40):
