@@ -15,6 +15,8 @@
 //           the chunk's border (at most two do) the sum is kept as a part.
 //   join    The chunk in which a crossing row starts adds the row's parts in order and stores it.
 // Bound by memory: the table's gradient is written once (V D elements) and again where a row has tokens, dy is read once.
+// 65536 tokens on 131072 x 1024 fp32: 106 us for the sort's launches with 512 MB of zeros beside it, 113 us for the chunks, 11 us
+// for the join; small tables are bound by the launches' latency (16384 tokens on 50001 x 1024 bf16: 38, 12 and 6 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
