@@ -474,7 +474,8 @@ DTF_EXPORT int dtf_embedding_bwd(const void* ids, int ids64, const void* dy, voi
   const int64_t bytes = V * D * (dtype == TK_BF16 ? 2 : 4), pieces = bytes / 16;
   const int shares = n <= kOne ? 1 : 2 * p.passes;
   auto fill = [&](int share) { return Fill{static_cast<tk_u32x4*>(out), (long)(pieces * share / shares), (long)(pieces * (share + 1) / shares)}; };
-  const unsigned fillers = (unsigned)std::min<int64_t>(511, (pieces / shares + kSortBlock - 1) / kSortBlock);
+  const int64_t most = (pieces + shares - 1) / shares;        // pieces of the largest share
+  const unsigned fillers = (unsigned)std::min<int64_t>(511, (most + kSortBlock - 1) / kSortBlock);
   if (bytes % 16) hipLaunchKernelGGL(emb_tail_kernel, dim3(1), dim3(64), 0, s, static_cast<char*>(out) + pieces * 16, (int)(bytes % 16));
   if (n <= kOne) {
     hipLaunchKernelGGL(emb_sort_one_kernel, dim3(1 + fillers), dim3(kSortBlock), 0, s, a, n > 0 ? p.passes : 0, fill(0));

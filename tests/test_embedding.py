@@ -86,6 +86,24 @@ def test_padding_index_and_id_types(idtype, dev):
 
 
 @pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("v,d", [(1, 1), (2, 2), (1, 4), (3, 2), (2, 8)])
+def test_tables_of_a_few_bytes_under_many_tokens(v, d, dev, monkeypatch):
+    """Fewer 16-byte pieces than the sort has launches: rows without tokens are zeros all the same."""
+    empty = torch.empty
+    # new memory may hold anything: here bytes of ones, NaN in either type
+    def poisoned(*args, **kw):
+        t = empty(*args, **kw)
+        t.view(torch.uint8).fill_(255)
+        return t
+
+    monkeypatch.setattr(torch, "empty", poisoned)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = em.embedding_bwd(torch.ones(10000, d, dtype=dtype, device=dev), torch.zeros(10000, dtype=torch.int64, device=dev), v)
+        assert torch.equal(got[1:], torch.zeros_like(got[1:]))
+        assert torch.equal(got[0].float(), torch.full((d,), 10000.0, device=dev).to(dtype).float())
+
+
+@pytest.mark.parametrize("dev", devices())
 def test_no_tokens_and_leading_axes(dev):
     table = torch.randn(11, 16, device=dev)
     y = em.embedding_fwd(torch.empty((0, 3), dtype=torch.int64, device=dev), table)
