@@ -425,7 +425,7 @@ void bwd_width(const LnBwdArgs& a, int parts, hipStream_t s) {
 DTF_EXPORT int dtf_layernorm_fwd(const void* x, const void* res, const void* w, const void* b, void* y, void* h, float* mean,
                                  float* rstd, int64_t rows, int C, int64_t ldx, int64_t ldres, int dtype, int w_dtype, float eps,
                                  hipStream_t s) {
-  if (rows < 0 || C <= 0 || rows > 0x7fffffffLL || ldx < C || (res && ldres < C)) return DTF_ERR_SHAPE;
+  if (rows < 0 || C <= 0 || C > (1 << 30) || rows > 0x7fffffffLL || ldx < C || (res && ldres < C)) return DTF_ERR_SHAPE;
   if ((dtype != TK_F32 && dtype != TK_BF16) || (w_dtype != TK_F32 && w_dtype != TK_BF16) || (res == nullptr) != (h == nullptr)) return DTF_ERR_ARG;
   if (rows == 0) return DTF_OK;
   if (!x || !y || !mean || !rstd) return DTF_ERR_ARG;
@@ -446,7 +446,7 @@ DTF_EXPORT int64_t dtf_layernorm_bwd_ws_floats(int64_t rows, int C) {
 DTF_EXPORT int dtf_layernorm_bwd(const void* dy, const void* h, const void* dh, const void* w, const float* mean, const float* rstd,
                                  void* dx, void* dw, void* db, float* part, int64_t rows, int C, int64_t lddy, int64_t ldh,
                                  int64_t lddh, int dtype, int w_dtype, hipStream_t s) {
-  if (rows < 0 || C <= 0 || rows > 0x7fffffffLL || lddy < C || ldh < C || (dh && lddh < C)) return DTF_ERR_SHAPE;
+  if (rows < 0 || C <= 0 || C > (1 << 30) || rows > 0x7fffffffLL || lddy < C || ldh < C || (dh && lddh < C)) return DTF_ERR_SHAPE;
   if ((dtype != TK_F32 && dtype != TK_BF16) || (w_dtype != TK_F32 && w_dtype != TK_BF16)) return DTF_ERR_ARG;
   const bool wgrad = dw || db;
   LnBwdArgs a = {dy, h, dh, w, mean, rstd, dx, part, (long)rows, C, (long)lddy, (long)ldh, (long)lddh, w_dtype, wgrad};

@@ -863,10 +863,11 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.ldd = up(a.D, 64);
   p.ldn = up(a.N, 64);
   // a piece: dz and its transpose in 1 GiB, but never under 16384 columns (the products' K and M); every operand of a
-  // launch stays below 2 GiB (32-bit offsets)
+  // launch stays below 2 GiB (32-bit offsets), and a launch of 128x128 blocks below 2^32 threads
   const long col = 2 * p.planes;                 // bytes an element of an operand takes
   long vp = backward ? std::max<long>((1l << 30) / (2 * col * p.ldn), 16384) : (1l << 30);
   vp = std::min(vp, ((1l << 31) - (1 << 20)) / (col * std::max({p.ldd, (long)a.ldw, backward ? p.ldn : 0})));
+  vp = std::min(vp, (1l << 37) / p.ldn);
   vp = std::max<long>(vp / 256 * 256, 256);
   p.pieces = (a.V + vp - 1) / vp;
   p.Vp = p.pieces == 1 ? a.V : std::min(vp, up((a.V + p.pieces - 1) / p.pieces, 256));

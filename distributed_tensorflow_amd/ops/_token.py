@@ -20,6 +20,12 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
+def at_most(what: str, n: int, most: int) -> None:
+    """Sizes that the C entry points take as 32-bit numbers: refused here, before they could wrap."""
+    if n > most:
+        raise ValueError(f"{what}: {n} is beyond the kernels' range of {most}")
+
+
 def same_device(what: str, first: torch.Tensor, *others) -> None:
     dev = first.device
     for t in others:

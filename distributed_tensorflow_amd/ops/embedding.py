@@ -21,7 +21,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, reference
-from ._token import DTYPES, dtype_code, launch, rows_2d, same_device
+from ._token import DTYPES, at_most, dtype_code, launch, rows_2d, same_device
 
 _protos_done = False
 
@@ -60,6 +60,7 @@ def embedding_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
     if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise ValueError("embedding: table must be [V, D]")
     dt = dtype_code(table, "embedding: table")
+    at_most("embedding: width of the table", table.shape[1], 1 << 20)
     same_device("embedding", table, ids)
     if not table.is_cuda:
         return reference.embedding(ids, table, scale)
@@ -77,6 +78,7 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, rows: int, scale: float =
     if rows <= 0 or dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
         raise ValueError(f"embedding_bwd: dy must be [*ids.shape, D], got {tuple(dy.shape)} for ids {tuple(ids.shape)}")
     dt, cols = dtype_code(dy, "embedding_bwd: dy"), dy.shape[-1]
+    at_most("embedding_bwd: width of the table", cols, 1 << 20)
     skip = _padding(padding_idx, rows)
     same_device("embedding_bwd", dy, ids)
     if not dy.is_cuda:

@@ -23,7 +23,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, reference
-from ._token import dtype_code, launch, rows_2d, same_device
+from ._token import at_most, dtype_code, launch, rows_2d, same_device
 
 _protos_done = False
 
@@ -81,6 +81,7 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("layer_norm: x needs a last axis of at least one element")
     dt, cols = dtype_code(x, "layer_norm: x"), x.shape[-1]
+    at_most("layer_norm: last axis", cols, 1 << 30)
     wcode = _param_code("layer_norm", x, weight, bias)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("layer_norm: residual must have x's shape and dtype")
@@ -110,6 +111,7 @@ def layer_norm_bwd(dy: torch.Tensor, fwd: LayerNormResult, weight: Optional[torc
     h = fwd.h
     cols = h.shape[-1]
     dt = dtype_code(h, "layer_norm_bwd: h")
+    at_most("layer_norm_bwd: last axis", cols, 1 << 30)
     wcode = _param_code("layer_norm_bwd", h, weight, None)
     for name, t in (("dy", dy), ("dh", dh)):
         if t is not None and (t.numel() != h.numel() or t.shape[-1] != cols or t.dtype != h.dtype):

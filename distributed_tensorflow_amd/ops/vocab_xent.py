@@ -26,7 +26,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, reference
-from ._token import DTYPES, dtype_code, launch, same_device
+from ._token import DTYPES, at_most, dtype_code, launch, same_device
 
 _protos_done = False
 REDUCTIONS = ("mean", "sum", "none")
@@ -88,6 +88,8 @@ def _check(features, weight, labels, bias):
         raise ValueError(f"vocab_xent: features [N, D] and weight [V, D], got {tuple(features.shape)} and {tuple(weight.shape)}")
     if weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError("vocab_xent: empty vocabulary or width")
+    at_most("vocab_xent: rows", features.shape[0], 1 << 26)
+    at_most("vocab_xent: width", features.shape[1], 1 << 20)
     code, wcode = dtype_code(features, "vocab_xent: features"), dtype_code(weight, "vocab_xent: weight")
     if wcode != code and wcode != 0:
         raise ValueError("vocab_xent: weight must have the features' dtype, or be float32")

@@ -173,6 +173,15 @@ def test_refusals(dev):
             call()
 
 
+@pytest.mark.parametrize("dev", devices())
+def test_a_width_of_more_than_32_bits_is_refused(dev):
+    ids, far = torch.zeros(1, dtype=torch.int64, device=dev), torch.zeros((1, 1), device=dev).expand(1, 2 ** 32 + 4)
+    with pytest.raises(ValueError, match="range"):
+        em.embedding_fwd(ids, far)
+    with pytest.raises(ValueError, match="range"):
+        em.embedding_bwd(far, ids, 3)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [3000, 30000])
 def test_same_bits_again_on_another_stream_and_in_replayed_graphs(n):

@@ -314,6 +314,32 @@ def test_refusals(dev):
             call()
 
 
+@pytest.mark.parametrize("dev", devices())
+def test_sizes_of_more_than_32_bits_are_refused(dev):
+    one = torch.zeros((1, 1), device=dev)
+    lab = torch.zeros(1, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError, match="range"):
+        vx.vocab_xent_fwd(one.expand(2 ** 32 + 4, 1), one, lab.expand(2 ** 32 + 4))
+    with pytest.raises(ValueError, match="range"):
+        vx.vocab_xent_fwd(one.expand(1, 2 ** 32 + 4), one.expand(3, 2 ** 32 + 4), lab)
+
+
+@pytest.mark.gpu
+def test_more_blocks_of_logits_than_one_launch_may_have():
+    """2^20 x 2^19 logits are 2^25 blocks of 128 x 128 and 2^33 threads; 64 distinct rows stand for all."""
+    n, v, d = 1 << 20, 1 << 19, 8
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, w = torch.randn((64, d), generator=g, device="cuda").bfloat16(), torch.randn((v, d), generator=g, device="cuda").bfloat16()
+    lab = torch.randint(0, v, (64,), generator=g, device="cuda")
+    r = vx.vocab_xent_fwd(x.repeat(n // 64, 1), w, lab.repeat(n // 64))
+    z = x.double() @ w.double().t()
+    want = torch.logsumexp(z, 1) - z.gather(1, lab[:, None])[:, 0]
+    # sum |x w| stays below 100, so a logit is off by at most 10 U32 * 100 = 6e-5; lse by that and 150 U32
+    assert float((x.double().abs() @ w.double().abs().t()).max()) < 100
+    assert float((r.loss_rows.double().reshape(-1, 64) - want).abs().max()) < 2e-4
+    assert int(r.count) == n and int(r.hits) == int((z.argmax(1) == lab).sum()) * (n // 64)
+
+
 @pytest.mark.gpu
 def test_operands_of_two_gibibytes_are_refused():
     x = torch.empty((1, 8), dtype=torch.bfloat16, device="cuda").expand(1 << 27, 8)

@@ -215,6 +215,13 @@ def test_refusals(dev):
             call()
 
 
+@pytest.mark.parametrize("dev", devices())
+def test_an_axis_of_more_than_32_bits_is_refused(dev):
+    """Not taken modulo 2^32."""
+    with pytest.raises(ValueError, match="range"):
+        ln.layer_norm(torch.zeros((1, 1), device=dev).expand(1, 2 ** 32 + 4))
+
+
 @pytest.mark.gpu
 def test_same_bits_again_on_another_stream_and_in_a_replayed_graph():
     x, dy = draw((700, 1024), torch.bfloat16).cuda(), draw((700, 1024), torch.bfloat16, 1).cuda()
