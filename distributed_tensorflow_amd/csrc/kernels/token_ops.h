@@ -101,7 +101,8 @@ __device__ __forceinline__ void tk_load_param(const void* p, int bf16, int c, in
     if (bf16) {
       const unsigned short* const q = static_cast<const unsigned short*>(p) + c;
       if constexpr (VEC == 8) {
-        TkVec<unsigned short, 8>::unpack(*reinterpret_cast<const tk_u32x4_at2*>(q), v);
+        const tk_u32x4 piece = *reinterpret_cast<const tk_u32x4_at2*>(q);
+        TkVec<unsigned short, 8>::unpack(piece, v);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = tk_bf2f(q[i]);
