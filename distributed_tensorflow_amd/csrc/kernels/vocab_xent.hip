@@ -80,9 +80,10 @@ struct alignas(16) VxRow {
 // exp(d) for d <= 0 or so with the rounding of d log2(e) made good: the product's error, up to |d| 2^-24 of the result, is
 // computed and applied to first order.
 __device__ __forceinline__ float exp_exact(float d) {
-  const float hi = d * 1.44269502f, lo = fmaf(d, 1.92596303e-8f, fmaf(d, 1.44269502f, -hi));
+  const float hi = d * 1.44269502f, rest = fmaf(d, 1.92596303e-8f, fmaf(d, 1.44269502f, -hi));
+  const float lo = d < -200.f ? 0.f : rest;      // there the result is 0, and of -inf the product's error is NaN
   const float e = __builtin_amdgcn_exp2f(hi);
-  return e > 0.f ? fmaf(e * 0.693147181f, lo, e) : e;              // 0 and NaN as they are
+  return fmaf(e * 0.693147181f, lo, e);
 }
 
 struct VxGemm : DtfGemmArgs {
@@ -207,7 +208,9 @@ struct VxGemm : DtfGemmArgs {
 #pragma unroll
           for (int cj = 0; cj < 4; ++cj) {
             const float d = acc[ri][cj][r] - row.top;
-            acc[ri][cj][r] = row.g == 0.f ? 0.f : (kF32Out ? exp_exact(d) : __expf(d)) * row.scaled;
+            float v = (kF32Out ? exp_exact(d) : __expf(d)) * row.scaled;
+            if (kF32Out) asm("" : "+v"(v));      // computed, then chosen: as a branch for every element it costs more
+            acc[ri][cj][r] = row.g == 0.f ? 0.f : v;
           }
         }
       }
@@ -549,10 +552,22 @@ __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short*
 
 // The three bf16 planes of an fp32 matrix [M, N] (any stride and alignment), straight [3][M, Np] and / or transposed
 // [3][Nt, Mp], zeros in the padding; in the transposed one also for rows without a gradient (see vx_transpose_kernel).
-__global__ __launch_bounds__(256) void vx_planes_kernel(const float* __restrict__ src, unsigned short* __restrict__ dst, unsigned short* __restrict__ dst_t,
-                                                        int M, int N, long lds_, int Np, int Nt, int Mp, const VxRow* __restrict__ rows) {
+// Two matrices a launch: those of a small X are latency only, beside W's they cost nothing.
+struct VxPlanes {
+  const float* src; unsigned short* dst; unsigned short* dst_t; const VxRow* rows;
+  long lds_; int M, N, Np, Nt, Mp, blocks;
+};
+__global__ __launch_bounds__(256) void vx_planes_kernel(VxPlanes first, VxPlanes second) {
+  const bool one = (int)blockIdx.x < first.blocks;
+  const float* const src = one ? first.src : second.src;
+  unsigned short* const dst = one ? first.dst : second.dst;
+  unsigned short* const dst_t = one ? first.dst_t : second.dst_t;
+  const VxRow* const rows = one ? first.rows : second.rows;
+  const long lds_ = one ? first.lds_ : second.lds_;
+  const int M = one ? first.M : second.M, N = one ? first.N : second.N, Np = one ? first.Np : second.Np, Nt = one ? first.Nt : second.Nt, Mp = one ? first.Mp : second.Mp;
+  const int block = (int)blockIdx.x - (one ? 0 : first.blocks);
   __shared__ float tile[64][65];
-  const int across = (Np + 63) >> 6, c0 = (int)(blockIdx.x % across) * 64, r0 = (int)(blockIdx.x / across) * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int across = (Np + 63) >> 6, c0 = block % across * 64, r0 = block / across * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int rr = ty + 4 * i;
@@ -602,11 +617,15 @@ __global__ __launch_bounds__(256) void vx_finish_kernel(const float* __restrict_
   const long i = (long)blockIdx.x * 256 + threadIdx.x, row = i / quads;
   const int c = (int)(i - row * quads) * 4;
   if (row >= rows) return;
-  f32x4 v = *reinterpret_cast<const f32x4*>(ws + (size_t)row * ldw + c);
-  for (int s = 1; s < splits; ++s) {
-    const f32x4 o = *reinterpret_cast<const f32x4*>(ws + ((size_t)s * rows + row) * ldw + c);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; s += 8) {          // eight loads under way at once (past the end: the last again, not added)
+    f32x4 o[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += o[e];
+    for (int u = 0; u < 8; ++u) o[u] = *reinterpret_cast<const f32x4*>(ws + ((size_t)min(s + u, splits - 1) * rows + row) * ldw + c);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += s + u < splits ? o[u][e] : 0.f;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -948,19 +967,23 @@ void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, 
   hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt, rows);
 }
 
-void planes(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, const VxRow* rows, hipStream_t s) {
-  const dim3 g((unsigned)(((Np + 63) / 64) * ((Mp + 63) / 64)));
-  hipLaunchKernelGGL(vx_planes_kernel, g, dim3(256), 0, s, static_cast<const float*>(src), static_cast<unsigned short*>(dst), static_cast<unsigned short*>(dst_t),
-                     (int)M, (int)N, lds_, (int)Np, (int)Nt, (int)Mp, rows);
+VxPlanes planes_of(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, const VxRow* rows) {
+  return {static_cast<const float*>(src), static_cast<unsigned short*>(dst), static_cast<unsigned short*>(dst_t), rows, lds_, (int)M, (int)N, (int)Np, (int)Nt, (int)Mp,
+          (int)(((Np + 63) / 64) * ((Mp + 63) / 64))};
+}
+// and leaves them empty
+void launch_planes(VxPlanes& a, VxPlanes& b, hipStream_t s) {
+  if (a.blocks + b.blocks) hipLaunchKernelGGL(vx_planes_kernel, dim3((unsigned)(a.blocks + b.blocks)), dim3(256), 0, s, a, b);
+  a.blocks = b.blocks = 0;
 }
 
 // One operand of the logits ([rows, D] of `from`, ld apart) as the kernel reads it, and transposed for a product (bf16: from
-// the aligned copy; to_t null: not needed).
+// the aligned copy; to_t null: not needed).  Planes are left to the caller to launch.
 struct Operand { const void* p; long ld; };
 Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int from, long rows, long ld, bool copy, void* dst, void* to_t, long ldt,
-                const VxRow* row_info, hipStream_t s) {
+                const VxRow* row_info, VxPlanes& planes, hipStream_t s) {
   Operand o = {src, ld};
-  if (!p.direct || (p.planes == 3 && to_t)) planes(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), row_info, s);
+  if (!p.direct || (p.planes == 3 && to_t)) planes = planes_of(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), row_info);
   if (p.direct && copy) pack(src, from, dst, a.dtype, rows, a.D, ld, p.ldd, s);
   if (copy) o = {dst, p.ldd};
   if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, row_info, s);
@@ -1020,11 +1043,13 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   if (a.ws_bytes < (int64_t)p.total) return DTF_ERR_SHAPE;
   if (!dtf_aligned16(a.ws)) return DTF_ERR_ALIGN;
   char* const ws = static_cast<char*>(a.ws);
-  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, nullptr, 0, nullptr, s);
+  VxPlanes of_x = {}, of_w = {};
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, nullptr, 0, nullptr, of_x, s);
   const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0);
-    const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w, nullptr, 0, nullptr, s);
+    const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w, nullptr, 0, nullptr, of_w, s);
+    launch_planes(of_x, of_w, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.labels = a.labels;
@@ -1053,14 +1078,16 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   const int Mp = (int)up(a.N, 256);
   float* const scale = reinterpret_cast<float*>(rows + Mp);
   hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.top, a.total, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, rows, scale);
-  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW && !p.small ? ws + p.xt : nullptr, p.ldn, rows, s);
+  VxPlanes of_x = {}, of_w = {};
+  const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW && !p.small ? ws + p.xt : nullptr, p.ldn, rows, of_x, s);
   const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
   float* const dx32 = reinterpret_cast<float*>(ws + p.dx32);
   float* const dw32 = reinterpret_cast<float*>(ws + p.dw32);
   for (long v0 = 0; v0 < a.V; v0 += p.Vp) {
     const long n = std::min<long>(p.Vp, a.V - v0), np = up(n, 8), ldv = up(n, 64);
     const Operand W = prepare(a, p, static_cast<const char*>(a.W) + v0 * a.ldw * (a.w_dtype == TK_BF16 ? 2 : 4), a.w_dtype, n, a.ldw, p.pack_w, ws + p.w,
-                              a.dX && !p.small ? ws + p.wt : nullptr, ldv, nullptr, s);
+                              a.dX && !p.small ? ws + p.wt : nullptr, ldv, nullptr, of_w, s);
+    launch_planes(of_x, of_w, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.rows = rows;
@@ -1072,7 +1099,10 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
     if (p.small) launch_small_dz(g, p.skinny, s);
     else launch_logits<VX_DZ>(g, p.skinny, s);
-    if (p.planes == 3 && !p.small) planes(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, nullptr, s);
+    if (p.planes == 3 && !p.small) {
+      VxPlanes none = {}, of_dz = planes_of(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, nullptr);
+      launch_planes(of_dz, none, s);
+    }
     if (a.dbias)
       hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
     if (p.small) {
