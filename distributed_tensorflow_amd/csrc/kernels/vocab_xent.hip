@@ -92,8 +92,8 @@ struct VxGemm : DtfGemmArgs {
   float2* part;                                  // [strips][M]
   float2* target;                                // [M]: the label's logit, whether an earlier column of its strip reaches it
   int v0;                                        // vocabulary index of column 0
-  // VX_DZ (C = dz [M, ldc], Ct = dz^T [N, ldct]; both leading dimensions are the padded widths, padding is zeroed; of fp32
-  // operands, and as VX_DZ32, only C, in fp32)
+  // VX_DZ (C = dz [M, ldc], Ct = dz^T [N, ldct], null: not needed; both leading dimensions are the padded widths, padding is
+  // zeroed; of fp32 operands three bf16 planes each); VX_DZ32: C in fp32
   const VxRow* rows;                             // padded to the block height
   unsigned a_plane, b_plane;                     // bytes between the planes of the operands (EPI_PLANES)
   float* db_part;                                // [wave rows][N], optional
@@ -130,7 +130,7 @@ struct VxGemm : DtfGemmArgs {
       store_sum<RI>(acc, wl, crow, ccol, lane);
       return;
     }
-    constexpr bool kF32Out = F32 || EPI == VX_DZ32;
+    constexpr bool kExact = F32 || EPI == VX_DZ32;
     const float NEG_INF = -__builtin_huge_valf();
     if (bias) {
 #pragma unroll
@@ -208,8 +208,8 @@ struct VxGemm : DtfGemmArgs {
 #pragma unroll
           for (int cj = 0; cj < 4; ++cj) {
             const float d = acc[ri][cj][r] - row.top;
-            float v = (kF32Out ? exp_exact(d) : __expf(d)) * row.scaled;
-            if (kF32Out) asm("" : "+v"(v));      // computed, then chosen: as a branch for every element it costs more
+            float v = (kExact ? exp_exact(d) : __expf(d)) * row.scaled;
+            if (kExact) asm("" : "+v"(v));      // computed, then chosen: as a branch for every element it costs more
             acc[ri][cj][r] = row.g == 0.f ? 0.f : v;
           }
         }
@@ -241,7 +241,7 @@ struct VxGemm : DtfGemmArgs {
           if (g == 0 && col < N) db_part[(size_t)(crow / (16 * RI)) * N + col] = v;
         }
       }
-      if constexpr (kF32Out) {
+      if constexpr (EPI == VX_DZ32) {
         float* const c = static_cast<float*>(C);
 #pragma unroll
         for (int ri = 0; ri < RI; ++ri)
@@ -253,18 +253,27 @@ struct VxGemm : DtfGemmArgs {
               if (row < M && col < ldc) c[(size_t)row * ldc + col] = acc[ri][cj][r];
             }
       } else {
-        store_dz<RI>(acc, wl, crow, ccol, lane);
+        if constexpr (!F32) {
+          store_dz<RI, false>(acc, wl, crow, ccol, lane, 0);
+        } else {
+#pragma unroll 1                                 // three planes at once would not fit the registers
+          for (int q = 0; q < 3; ++q) {
+            int l = lane;
+            asm volatile("" : "+v"(l));          // addresses are computed plane by plane, not kept
+            store_dz<RI, true>(acc, wl, crow, ccol, l, q);
+          }
+        }
       }
     }
   }
 
   // Both images are turned in LDS, so that every global store is 16 bytes a lane.
-  template <int RI>
-  __device__ __forceinline__ void store_dz(const f32x4 (&acc)[RI][4], unsigned char* wl, int crow, int ccol, int lane) const {
+  template <int RI, bool PLANES>
+  __device__ __forceinline__ void store_dz(f32x4 (&acc)[RI][4], unsigned char* wl, int crow, int ccol, int lane, int plane) const {
     constexpr int CH = 2 * RI;                   // 16-byte chunks of a transposed row (16 RI rows of dz)
     const int fr = lane & 15, g = lane >> 4;
-    unsigned short* const c = static_cast<unsigned short*>(C);
-    unsigned short* const ct = static_cast<unsigned short*>(Ct);
+    unsigned short* const c = static_cast<unsigned short*>(C) + (size_t)plane * M * ldc;
+    unsigned short* const ct = static_cast<unsigned short*>(Ct) + (size_t)plane * N * ldct;
     uint2 pk[RI][4];
 #pragma unroll
     for (int ri = 0; ri < RI; ++ri)
@@ -272,20 +281,28 @@ struct VxGemm : DtfGemmArgs {
       for (int cj = 0; cj < 4; ++cj) {
         pk[ri][cj].x = tk_pack2(acc[ri][cj][0], acc[ri][cj][1]);
         pk[ri][cj].y = tk_pack2(acc[ri][cj][2], acc[ri][cj][3]);
+        if (PLANES) {                            // what the next planes hold; now, so that nothing else stays alive
+          acc[ri][cj][0] -= __uint_as_float(pk[ri][cj].x << 16); acc[ri][cj][1] -= __uint_as_float(pk[ri][cj].x & 0xffff0000u);
+          acc[ri][cj][2] -= __uint_as_float(pk[ri][cj].y << 16); acc[ri][cj][3] -= __uint_as_float(pk[ri][cj].y & 0xffff0000u);
+          asm volatile("" : "+v"(acc[ri][cj]));
+        }
       }
+    if (Ct) {
 #pragma unroll
-    for (int ri = 0; ri < RI; ++ri)
+      for (int ri = 0; ri < RI; ++ri)
 #pragma unroll
-      for (int cj = 0; cj < 4; ++cj) {
-        const int col = 16 * cj + fr, q = 2 * ri + (g >> 1);
-        *reinterpret_cast<uint2*>(&wl[col * CH * 16 + ((q ^ (col & (CH - 1))) << 4) + 8 * (g & 1)]) = pk[ri][cj];
+        for (int cj = 0; cj < 4; ++cj) {
+          const int col = 16 * cj + fr, q = 2 * ri + (g >> 1);
+          *reinterpret_cast<uint2*>(&wl[col * CH * 16 + ((q ^ (col & (CH - 1))) << 4) + 8 * (g & 1)]) = pk[ri][cj];
+        }
+#pragma unroll
+      for (int it = 0; it < CH; ++it) {
+        const int col = it * (64 / CH) + lane / CH, q = lane & (CH - 1);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(&wl[col * CH * 16 + ((q ^ (col & (CH - 1))) << 4)]);
+        if (ccol + col < N && crow + q * 8 < ldct) *reinterpret_cast<u32x4*>(&ct[(size_t)(ccol + col) * ldct + crow + q * 8]) = v;
       }
-#pragma unroll
-    for (int it = 0; it < CH; ++it) {
-      const int col = it * (64 / CH) + lane / CH, q = lane & (CH - 1);
-      const u32x4 v = *reinterpret_cast<const u32x4*>(&wl[col * CH * 16 + ((q ^ (col & (CH - 1))) << 4)]);
-      if (ccol + col < N && crow + q * 8 < ldct) *reinterpret_cast<u32x4*>(&ct[(size_t)(ccol + col) * ldct + crow + q * 8]) = v;
     }
+    if (!C) return;
     // straight image: neighbouring lanes swap halves, so that a lane holds two rows of two neighbouring columns and writes
     // 32-bit pieces (even lanes rows 0 and 1 of the four, odd lanes rows 2 and 3)
     const bool odd = fr & 1;
@@ -922,7 +939,6 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
     } else {
       p.xt = take(at, (size_t)p.Dp * p.ldn * col);
       p.wt = take(at, (size_t)p.Dp * p.ldv * col);
-      if (p.planes == 3) p.dz32 = take(at, (size_t)a.N * p.ldv * 4);
       p.dz = take(at, (size_t)a.N * p.ldv * col);
       p.dzt = take(at, (size_t)p.Vp * p.ldn * col);
       p.sx = splits_for(p.planes, a.N, p.Dp, Vpp);
@@ -992,8 +1008,9 @@ Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int
 
 // dz in fp32 for the kernels of few rows
 void launch_small_dz(const VxGemm& a, bool skinny, hipStream_t s) {
-  if (a.dtype == TK_F32) launch_logits<VX_DZ>(a, skinny, s);           // fp32 operands leave fp32
-  else if (skinny) launch_skinny<VX_DZ32>(a, s);
+  if (skinny) launch_skinny<VX_DZ32>(a, s);
+  else if (a.dtype == TK_F32)
+    hipLaunchKernelGGL((gemm_tiled_kernel<unsigned int, VX_DZ32, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, VX_DZ32, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
 }
 
@@ -1092,17 +1109,13 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.bias = a.bias ? a.bias + v0 : nullptr;
     g.rows = rows;
     g.v0 = (int)v0;
-    g.C = ws + (p.planes == 3 || p.small ? p.dz32 : p.dz);
+    g.C = p.small ? ws + p.dz32 : a.dX ? ws + p.dz : nullptr;
     g.ldc = (int)ldv;
-    g.Ct = ws + p.dzt;
+    g.Ct = a.dW && !p.small ? ws + p.dzt : nullptr;
     g.ldct = (int)p.ldn;
     g.db_part = a.dbias ? reinterpret_cast<float*>(ws + p.db) : nullptr;
     if (p.small) launch_small_dz(g, p.skinny, s);
     else launch_logits<VX_DZ>(g, p.skinny, s);
-    if (p.planes == 3 && !p.small) {
-      VxPlanes none = {}, of_dz = planes_of(ws + p.dz32, a.dX ? ws + p.dz : nullptr, a.dW ? ws + p.dzt : nullptr, a.N, n, ldv, ldv, n, p.ldn, nullptr);
-      launch_planes(of_dz, none, s);
-    }
     if (a.dbias)
       hipLaunchKernelGGL(vx_db_kernel, dim3(dtf_cdiv((int)n, 256)), dim3(256), 0, s, g.db_part, dtf_cdiv(a.N, wave_rows(g, p.skinny)), (int)n, a.dbias + v0, scale);
     if (p.small) {

@@ -315,6 +315,19 @@ def test_refusals(dev):
 
 
 @pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v", [(20, 100), (100, 300), (300, 16400)])
+def test_selected_gradients_are_those_of_a_full_call(n, v, dtype, dev):
+    x, w, lab, b = (t.to(dev) for t in draw(n, v, 40, dtype))
+    r = vx.vocab_xent_fwd(x, w, lab, b)
+    full = vx.vocab_xent_bwd(r, x, w, lab, b)
+    for k in range(1, 8):
+        want = [bool(k >> i & 1) for i in range(3)]
+        for got, one, take in zip(vx.vocab_xent_bwd(r, x, w, lab, b, want=want), full, want):
+            assert torch.equal(got, one) if take else got is None
+
+
+@pytest.mark.parametrize("dev", devices())
 def test_sizes_of_more_than_32_bits_are_refused(dev):
     one = torch.zeros((1, 1), device=dev)
     lab = torch.zeros(1, dtype=torch.int64, device=dev)
