@@ -371,53 +371,85 @@ struct VxGemm : DtfGemmArgs {
   }
 };
 
-// Few rows, or few columns: 16 rows x 64 columns a workgroup, the four waves share K (64 bytes of a row a step, wave by
-// wave), operands straight from memory into the matrix instructions: one wave's 20 loads in flight, no staging, no barrier
-// in the loop.  Every row of W is read by ceil(M / 16) workgroups, next to each other on one XCD.
-template <typename T, int EPI>
+// Few rows, or few columns: 16 RT rows x 64 columns a workgroup, the four waves share K (64 bytes of a row a step, wave by
+// wave), operands straight from memory into the matrix instructions: one wave's 16 to 24 loads in flight, no staging, no
+// barrier in the loop.  Every row of W is read by ceil(M / 16 RT) workgroups, next to each other on one XCD.
+// Not ALIGNED (fp32 only): rows of any width, stride and alignment, the elements behind a row's end replaced by zeros.
+template <typename T, int EPI, int RT, bool ALIGNED>
 __global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
-  constexpr int PER16 = Elem<T>::PER16, AHEAD = 4;
-  __shared__ float s_acc[3][16][64];
-  __shared__ __attribute__((aligned(16))) unsigned char s_out[2048];
+  typedef std::conditional_t<sizeof(T) == 4, float, unsigned short> E;
+  constexpr int PER16 = Elem<T>::PER16, AHEAD = RT == 4 ? 2 : 4;
+  __shared__ float s_acc[3][16 * RT][64];
+  __shared__ __attribute__((aligned(16))) unsigned char s_out[2048 * RT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
-  const int tiles_m = (p.M + 15) >> 4, wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
-  const int m0 = (wg % tiles_m) * 16, n0 = (wg / tiles_m) * 64;
+  const int tiles_m = (p.M + 16 * RT - 1) / (16 * RT), wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
+  const int m0 = (wg % tiles_m) * 16 * RT, n0 = (wg / tiles_m) * 64;
   const rsrc_t ra = make_rsrc(p.A, p.a_bytes), rb = make_rsrc(p.B, p.b_bytes);
-  const unsigned a_off = m0 + fr < p.M ? (unsigned)(m0 + fr) * (unsigned)p.lda * (unsigned)sizeof(T) : kOOB;
-  unsigned b_off[4];
+  // rows and columns past the last repeat it: the epilogue leaves them out
+  unsigned a_off[RT], b_off[4];
+  const E* a_row[RT];
+  const E* b_row[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b_off[j] = n0 + 16 * j + fr < p.N ? (unsigned)(n0 + 16 * j + fr) * (unsigned)p.ldb * (unsigned)sizeof(T) : kOOB;
-  f32x4 acc[1][4];
+  for (int i = 0; i < RT; ++i) {
+    const int row = min(m0 + 16 * i + fr, p.M - 1);
+    a_off[i] = (unsigned)row * (unsigned)p.lda * (unsigned)sizeof(T);
+    a_row[i] = static_cast<const E*>(p.A) + (long)row * p.lda;
+  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < 4; ++j) {
+    const int row = min(n0 + 16 * j + fr, p.N - 1);
+    b_off[j] = (unsigned)row * (unsigned)p.ldb * (unsigned)sizeof(T);
+    b_row[j] = static_cast<const E*>(p.B) + (long)row * p.ldb;
+  }
+  f32x4 acc[RT][4];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int steps = (p.K + 4 * PER16 - 1) / (4 * PER16);
   for (int s = wave; s < steps; s += 4 * AHEAD) {
-    u32x4 a[AHEAD], b[AHEAD][4];
+    u32x4 a[AHEAD][RT], b[AHEAD][4];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int k = (s + 4 * u) * 4 + g;           // 16-byte piece of the row
       const bool in = k * PER16 < p.K;
-      a[u] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(in && a_off != kOOB ? a_off + k * 16u : kOOB), 0, 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(in && b_off[j] != kOOB ? b_off[j] + k * 16u : kOOB), 0, 0);
+      for (int i = 0; i < RT; ++i) {
+        if constexpr (ALIGNED) a[u][i] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(in ? a_off[i] + k * 16u : kOOB), 0, 0);
+        else a[u][i] = in ? TkPiece<E, false>::load(a_row[i], k * PER16, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (ALIGNED) b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(in ? b_off[j] + k * 16u : kOOB), 0, 0);
+        else b[u][j] = in ? TkPiece<E, false>::load(b_row[j], k * PER16, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+      }
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma_slot<T>(a[u], b[u][j], acc[0][j]);
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma_slot<T>(a[u][i], b[u][j], acc[i][j]);
   }
   if (wave) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s_acc[wave - 1][4 * j + r][lane] = acc[0][j][r];
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_acc[wave - 1][16 * i + 4 * j + r][lane] = acc[i][j][r];
   }
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[0][j][r] = ((acc[0][j][r] + s_acc[0][4 * j + r][lane]) + s_acc[1][4 * j + r][lane]) + s_acc[2][4 * j + r][lane];
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 16 * i + 4 * j + r;
+        acc[i][j][r] = ((acc[i][j][r] + s_acc[0][at][lane]) + s_acc[1][at][lane]) + s_acc[2][at][lane];
+      }
   p.template epilogue<EPI, sizeof(T) == 4>(acc, s_out, m0, n0, lane);
 }
 
@@ -425,28 +457,33 @@ __global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
 // into reading W and writing dW once, so no transposed copies and no planes are made.  A lane's 16-byte piece of a row of W
 // (or X) is the operand of VEC instructions at once: instruction q takes column c0 + VEC fr + q.
 
-// dX: workgroup (column tile, 16 rows, range of the vocabulary); the waves take 16 vocabulary rows each in turn.
+// dX: workgroup (column tile, 16 RT rows, range of the vocabulary); the waves take 16 vocabulary rows each in turn.
 // ROUND: fp32 weights under bf16 activations, rounded as the logits' copy of them was.
-template <typename T, bool ROUND>
+template <typename T, bool ROUND, int RT>
 __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restrict__ dz, long lddz, const T* __restrict__ w, long ldw, float* __restrict__ out,
                                                           int M, int D, long n, int per, int ldo) {
   typedef TkPiece<T, false> P;
   constexpr int VEC = P::VEC;
-  __shared__ float s_acc[3][4 * VEC][64];
+  __shared__ float s_acc[3][4 * VEC * RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int c = (int)blockIdx.x * 16 * VEC + VEC * fr, m0 = blockIdx.y * 16;
+  const int c = (int)blockIdx.x * 16 * VEC + VEC * fr, m0 = blockIdx.y * 16 * RT;
   const long lo = (long)blockIdx.z * per, hi = min(n, lo + per);
-  f32x4 acc[VEC];
+  f32x4 acc[RT][VEC];
+  const float* arow[RT];                         // rows past the last repeat it and are not stored
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float* const arow = dz + (long)(m0 + fr < M ? m0 + fr : 0) * lddz;
+  for (int i = 0; i < RT; ++i) {
+    arow[i] = dz + (long)min(m0 + 16 * i + fr, M - 1) * lddz;
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   for (long v = lo + 16 * wave; v < hi; v += 128) {
-    f32x4 a[2];
+    f32x4 a[2][RT];
     tk_u32x4 b[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const long at = v + 64 * u + 4 * g;        // dz is zero from n to its padded width, a multiple of 64 columns
-      a[u] = v + 64 * u < hi && m0 + fr < M ? *reinterpret_cast<const f32x4*>(arow + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[u][i] = v + 64 * u < hi ? *reinterpret_cast<const f32x4*>(arow[i] + at) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 4; ++j) b[u][j] = at + j < hi && c < D ? P::load(w + (at + j) * ldw, c, D) : tk_u32x4{0u, 0u, 0u, 0u};
     }
@@ -459,54 +496,64 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
           if (ROUND) wv[q] = tk_bf2f(tk_f2bf(wv[q]));
-          acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][j], wv[q], acc[q], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i][j], wv[q], acc[i][q], 0, 0, 0);
         }
       }
   }
   if (wave) {
 #pragma unroll
-    for (int q = 0; q < VEC; ++q)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s_acc[wave - 1][4 * q + r][lane] = acc[q][r];
+      for (int q = 0; q < VEC; ++q)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_acc[wave - 1][4 * (VEC * i + q) + r][lane] = acc[i][q][r];
   }
   __syncthreads();
   if (wave || c >= ldo) return;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = m0 + 4 * g + r;
-    if (row >= M) continue;
-    float* const o = out + ((size_t)blockIdx.z * M + row) * ldo + c;
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int q = 0; q < VEC; q += 4) {
-      f32x4 t;
+    for (int r = 0; r < 4; ++r) {
+      const int row = m0 + 16 * i + 4 * g + r;
+      if (row >= M) continue;
+      float* const o = out + ((size_t)blockIdx.z * M + row) * ldo + c;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        t[e] = ((acc[q + e][r] + s_acc[0][4 * (q + e) + r][lane]) + s_acc[1][4 * (q + e) + r][lane]) + s_acc[2][4 * (q + e) + r][lane];
-      if (c + q < ldo) *reinterpret_cast<f32x4*>(o + q) = t;
+      for (int q = 0; q < VEC; q += 4) {
+        f32x4 t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = 4 * (VEC * i + q + e) + r;
+          t[e] = ((acc[i][q + e][r] + s_acc[0][at][lane]) + s_acc[1][at][lane]) + s_acc[2][at][lane];
+        }
+        if (c + q < ldo) *reinterpret_cast<f32x4*>(o + q) = t;
+      }
     }
-  }
 }
 
-// dW: a wave owns 16 vocabulary rows and 16 VEC columns.
-template <typename TX, typename TO>
+// dW: a wave owns 16 RT vocabulary rows and 16 VEC columns; the waves of a workgroup have the columns in common.
+template <typename TX, typename TO, int RT>
 __global__ __launch_bounds__(256) void vx_small_dw_kernel(const float* __restrict__ dz, long lddz, const TX* __restrict__ x, long ldx, TO* __restrict__ out,
                                                           int M, int D, long n, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
   typedef TkPiece<TX, false> P;
   constexpr int VEC = P::VEC, OUT = 16 / sizeof(TO);
   const int lane = threadIdx.x & 63, fr = lane & 15, g = lane >> 4;
   const int tiles = (D + 16 * VEC - 1) / (16 * VEC);
-  const long v0 = (long)(blockIdx.x / tiles) * 64 + 16 * (threadIdx.x >> 6);
+  const long v0 = (long)(blockIdx.x / tiles) * 64 * RT + 16 * RT * (threadIdx.x >> 6);
   const int c = (int)(blockIdx.x % tiles) * 16 * VEC + VEC * fr;
-  f32x4 acc[VEC];
+  f32x4 acc[RT][VEC];
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < M; k += 16) {
-    float a[4];
+    float a[4][RT];
     tk_u32x4 b[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int row = k + 4 * u + g;
-      a[u] = row < M && v0 + fr < n ? dz[(long)row * lddz + v0 + fr] : 0.f;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[u][i] = row < M && v0 + 16 * i + fr < n ? dz[(long)row * lddz + v0 + 16 * i + fr] : 0.f;
       b[u] = row < M && c < D && rows[row].g != 0.f ? P::load(x + (long)row * ldx, c, D) : tk_u32x4{0u, 0u, 0u, 0u};       // (see vx_transpose_kernel)
     }
 #pragma unroll
@@ -514,22 +561,26 @@ __global__ __launch_bounds__(256) void vx_small_dw_kernel(const float* __restric
       float xv[VEC];
       P::unpack(b[u], xv);
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u], xv[q], acc[q], 0, 0, 0);
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i], xv[q], acc[i][q], 0, 0, 0);
     }
   }
   const float f = *scale;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const long v = v0 + 4 * g + r;
-    if (v >= n) continue;
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int q = 0; q < VEC; q += OUT) {
-      float t[OUT];
+    for (int r = 0; r < 4; ++r) {
+      const long v = v0 + 16 * i + 4 * g + r;
+      if (v >= n) continue;
 #pragma unroll
-      for (int e = 0; e < OUT; ++e) t[e] = acc[q + e][r] * f;
-      if (c + q < D) TkPiece<TO, false>::store(out + v * D, c + q, D, t);
+      for (int q = 0; q < VEC; q += OUT) {
+        float t[OUT];
+#pragma unroll
+        for (int e = 0; e < OUT; ++e) t[e] = acc[i][q + e][r] * f;
+        if (c + q < D) TkPiece<TO, false>::store(out + v * D, c + q, D, t);
+      }
     }
-  }
 }
 
 // ------------------------------------------------------------------------------------------------- streaming helpers
@@ -792,28 +843,33 @@ bool use_pp(int planes, long m, long n, long k, int splits) {
   return m >= 256 && n >= 256 && k / splits >= 256 && blocks >= (deep >= 2048 ? 112 : 192);
 }
 
-// Up to so many rows the products read W and X as they are (vx_small_dx_kernel, vx_small_dw_kernel).  Backward pass at
-// 131072 x 4096, this way / through transposed copies: bf16 32 rows 1.04 / 1.21 ms, 64 rows 1.65 / 1.22; fp32 64 rows 3.4 / 5.3.
-bool use_small(int dtype, long m) { return m <= (dtype == TK_BF16 ? 32 : 64); }
+// Up to so many rows the products read W and X as they are (vx_small_dx_kernel, vx_small_dw_kernel).
+bool use_small(int dtype, long m) { return dtype == TK_BF16 ? m <= 32 : m < 256; }
 
 // Logits by the kernel that shares K between the waves: where 128x128 blocks would leave most CUs idle or, with few rows, be
 // mostly empty (bf16: as long as W is small; a large one streams faster through the 128x128 blocks: 131072 x 4096, one row,
-// 203 against 227 us); fp32 with few rows always (its 128x128 blocks compute 128 rows at a
-// sixteenth of the bf16 rate: 1.1 ms for 131072 x 4096, which three tiles of 16 rows reach).
+// 203 against 227 us); fp32 with fewer rows than planes pay for always.
 bool use_skinny(int dtype, long m, long n) {
   const long blocks = ((m + 127) / 128) * ((n + 127) / 128);
-  return blocks < 128 || (dtype == TK_F32 ? m <= 48 : m <= 16 && blocks < 512);
+  return blocks < 128 || (dtype == TK_F32 ? m < 256 : m <= 16 && blocks < 512);
 }
 
-// fp32 logits from planes: they cost 10 bytes of traffic for every element of W, which pays from about 256 rows on (131072 x
-// 4096, 64 rows: 2.5 ms through planes).
-bool use_planes(int dtype, long m, bool skinny) { return dtype == TK_F32 && !skinny && m >= 256; }
+// fp32 logits from planes: they cost 10 bytes of traffic for every element of W, which pays from about 256 rows on.
+bool use_planes(int dtype, bool skinny) { return dtype == TK_F32 && !skinny; }
 
-// fp32 operands as they are
-bool direct_f32(const VxGemm& a) { return a.dtype == TK_F32 && a.a_plane == 0; }
+// Tiles of 16 rows that one workgroup of the kernels of few rows takes (each element of W it reads serves all of them), as
+// long as two workgroups a CU are left.
+int row_tiles(int dtype, long m, long others) {
+  for (int rt = dtype == TK_BF16 ? 2 : 4; rt > 1; rt /= 2)
+    if (m > 8 * rt && (m + 16 * rt - 1) / (16 * rt) * others >= 512) return rt;
+  return 1;
+}
+int skinny_tiles(int dtype, long m, long n) { return dtype == TK_BF16 ? 1 : row_tiles(dtype, m, (n + 63) / 64); }
 
 // Rows of a wave's block in the logits' epilogue
-int wave_rows(const VxGemm& a, bool skinny) { return skinny ? 16 : direct_f32(a) ? 64 : use_pp(a.a_plane ? 3 : 1, a.M, a.N, a.K, 1) ? 128 : 64; }
+int wave_rows(const VxGemm& a, bool skinny) {
+  return skinny ? 16 * skinny_tiles(a.dtype, a.M, a.N) : use_pp(a.a_plane ? 3 : 1, a.M, a.N, a.K, 1) ? 128 : 64;
+}
 
 template <int EPI>
 void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
@@ -829,18 +885,29 @@ void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
   }
 }
 
+template <int EPI, int RT>
+void launch_skinny_f32(const VxGemm& a, hipStream_t s) {
+  const dim3 g((unsigned)(dtf_cdiv(a.M, 16 * RT) * dtf_cdiv(a.N, 64)));
+  const bool aligned = a.K % 4 == 0 && a.lda % 4 == 0 && a.ldb % 4 == 0 && dtf_aligned16(a.A) && dtf_aligned16(a.B);
+  if (aligned) hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, RT, true>), g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, RT, false>), g, dim3(256), 0, s, a);
+}
 template <int EPI>
 void launch_skinny(const VxGemm& a, hipStream_t s) {
-  const dim3 g((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64)));
-  if (a.dtype == TK_BF16) hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI>), g, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI>), g, dim3(256), 0, s, a);
+  if (a.dtype == TK_BF16) {
+    hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI, 1, true>), dim3((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64))), dim3(256), 0, s, a);
+    return;
+  }
+  switch (skinny_tiles(a.dtype, a.M, a.N)) {
+    case 1: launch_skinny_f32<EPI, 1>(a, s); break;
+    case 2: launch_skinny_f32<EPI, 2>(a, s); break;
+    default: launch_skinny_f32<EPI, 4>(a, s);
+  }
 }
 
 template <int EPI>
 void launch_logits(const VxGemm& a, bool skinny, hipStream_t s) {
   if (skinny) launch_skinny<EPI>(a, s);
-  else if (direct_f32(a))
-    hipLaunchKernelGGL((gemm_tiled_kernel<unsigned int, EPI, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
   else launch_gemm<EPI>(a, 1, s);
 }
 
@@ -880,6 +947,7 @@ struct VxPlan {
   int K;                                         // of the logits: padded only where both operands are
   int planes;                                    // of every operand of the large products
   bool skinny, direct, small, pack_x, pack_w, direct_dx, direct_dw;       // direct: the logits read X and W (or padded copies) as they are
+  int rt;                                        // of few rows: tiles of 16 rows a workgroup of dX
   int sx, sw;                                    // splits of the two products
   size_t x, w, part, target, blk, rows, xt, wt, dz32, dz, dzt, dx32, dw32, db, total;
 };
@@ -892,7 +960,7 @@ size_t take(size_t& at, size_t bytes) {
 
 VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   VxPlan p = {};
-  const long es = a.dtype == TK_BF16 ? 2 : 4, per16 = 16 / es;
+  const long es = a.dtype == TK_BF16 ? 2 : 4;
   p.planes = a.dtype == TK_BF16 ? 1 : 3;
   p.Dp = up(a.D, 8);
   p.Np = up(a.N, 8);
@@ -910,13 +978,14 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.pieces = (a.V + p.Vp - 1) / p.Vp;
   p.ldv = up(p.Vp, 64);
   p.skinny = use_skinny(a.dtype, a.N, p.Vp);
-  p.direct = !use_planes(a.dtype, a.N, p.skinny);
+  p.direct = !use_planes(a.dtype, p.skinny);
   p.small = use_small(a.dtype, a.N);
-  // copies where the operand's rows are no whole aligned 16-byte pieces, or planes
-  const bool odd_x = a.D % per16 || a.ldx % per16 || !dtf_aligned16(a.X), odd_w = a.D % per16 || a.ldw % per16 || !dtf_aligned16(a.W);
-  p.K = p.direct && a.D % per16 == 0 ? a.D : (int)p.Dp;
-  p.pack_x = p.direct ? odd_x : true;
-  p.pack_w = p.direct ? odd_w || a.w_dtype != a.dtype : true;
+  // copies: planes, or bf16 rows that are no whole aligned 16-byte pieces
+  const bool bf16 = a.dtype == TK_BF16;
+  const bool odd_x = a.D % 8 || a.ldx % 8 || !dtf_aligned16(a.X), odd_w = a.D % 8 || a.ldw % 8 || !dtf_aligned16(a.W);
+  p.K = p.direct && (!bf16 || a.D % 8 == 0) ? a.D : (int)p.Dp;
+  p.pack_x = !p.direct || (bf16 && odd_x);
+  p.pack_w = !p.direct || (bf16 && (odd_w || a.w_dtype != a.dtype));
   const size_t copy = p.direct ? es : 6;
   size_t at = 0;
   if (p.pack_x) p.x = take(at, (size_t)a.N * p.ldd * copy);
@@ -933,8 +1002,10 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
     if (p.small) {
       p.dz32 = take(at, (size_t)a.N * p.ldv * 4);
       // column tiles x row tiles x ranges of the vocabulary: about 1024 workgroups, ranges of 256 or more
-      const long tiles = ((a.D + 16 * (a.w_dtype == TK_BF16 ? 8 : 4) - 1) / (16 * (a.w_dtype == TK_BF16 ? 8 : 4))) * ((a.N + 15) / 16);
-      p.sx = (int)std::max<long>(1, std::min<long>({1024 / tiles, p.Vp / 256, 256}));
+      const int cols = a.w_dtype == TK_BF16 ? 128 : 64;
+      const long tiles = (a.D + cols - 1) / cols, ranges = std::max<long>(1, std::min<long>(p.Vp / 256, 256));
+      p.rt = row_tiles(a.w_dtype, a.N, tiles * ranges);
+      p.sx = (int)std::max<long>(1, std::min<long>(1024 / (tiles * ((a.N + 16 * p.rt - 1) / (16 * p.rt))), ranges));
       p.dx32 = take(at, (size_t)p.pieces * p.sx * a.N * p.Dp * 4);
     } else {
       p.xt = take(at, (size_t)p.Dp * p.ldn * col);
@@ -972,9 +1043,8 @@ void pack_as(const void* src, void* dst, long rows, int cols, long lds_, long ld
   hipLaunchKernelGGL((vx_pack_kernel<TS, TD>), dim3((unsigned)((rows * ldd + 255) / 256)), dim3(256), 0, s, static_cast<const TS*>(src),
                      static_cast<TD*>(dst), (int)rows, cols, lds_, (int)ldd);
 }
-void pack(const void* src, int sdt, void* dst, int ddt, long rows, int cols, long lds_, long ldd, hipStream_t s) {
-  if (ddt == TK_F32) pack_as<float, float>(src, dst, rows, cols, lds_, ldd, s);
-  else if (sdt == TK_F32) pack_as<float, unsigned short>(src, dst, rows, cols, lds_, ldd, s);
+void pack(const void* src, int sdt, void* dst, long rows, int cols, long lds_, long ldd, hipStream_t s) {
+  if (sdt == TK_F32) pack_as<float, unsigned short>(src, dst, rows, cols, lds_, ldd, s);
   else pack_as<unsigned short, unsigned short>(src, dst, rows, cols, lds_, ldd, s);
 }
 
@@ -1000,7 +1070,7 @@ Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int
                 const VxRow* row_info, VxPlanes& planes, hipStream_t s) {
   Operand o = {src, ld};
   if (!p.direct || (p.planes == 3 && to_t)) planes = planes_of(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), row_info);
-  if (p.direct && copy) pack(src, from, dst, a.dtype, rows, a.D, ld, p.ldd, s);
+  if (p.direct && copy) pack(src, from, dst, rows, a.D, ld, p.ldd, s);
   if (copy) o = {dst, p.ldd};
   if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, row_info, s);
   return o;
@@ -1009,30 +1079,39 @@ Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int
 // dz in fp32 for the kernels of few rows
 void launch_small_dz(const VxGemm& a, bool skinny, hipStream_t s) {
   if (skinny) launch_skinny<VX_DZ32>(a, s);
-  else if (a.dtype == TK_F32)
-    hipLaunchKernelGGL((gemm_tiled_kernel<unsigned int, VX_DZ32, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((gemm_tiled_kernel<unsigned short, VX_DZ32, 4, 4, VxGemm>), dim3(dtf_cdiv(a.M, 128) * dtf_cdiv(a.N, 128)), dim3(256), 0, s, a);
 }
 
-void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
-  const int vec = a.w_dtype == TK_BF16 ? 8 : 4;
+template <typename T, bool ROUND, int RT>
+void small_dx_as(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
+  const dim3 g((unsigned)dtf_cdiv(a.D, 256 / (int)sizeof(T)), (unsigned)dtf_cdiv(a.N, 16 * RT), (unsigned)p.sx);
   const int per = (int)up((p.Vp + p.sx - 1) / p.sx, 64);
-  const dim3 g((unsigned)dtf_cdiv(a.D, 16 * vec), (unsigned)dtf_cdiv(a.N, 16), (unsigned)p.sx);
-  auto go = [&](auto kernel, auto* wt) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, dz, lddz, wt, (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp); };
-  if (a.w_dtype == TK_BF16) go(vx_small_dx_kernel<unsigned short, false>, static_cast<const unsigned short*>(w));
-  else if (a.dtype == TK_BF16) go(vx_small_dx_kernel<float, true>, static_cast<const float*>(w));
-  else go(vx_small_dx_kernel<float, false>, static_cast<const float*>(w));
+  hipLaunchKernelGGL((vx_small_dx_kernel<T, ROUND, RT>), g, dim3(256), 0, s, dz, lddz, static_cast<const T*>(w), (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp);
+}
+template <typename T, bool ROUND>
+void small_dx_of(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
+  if (p.rt == 1) small_dx_as<T, ROUND, 1>(a, p, dz, lddz, w, n, out, s);
+  else if (p.rt == 2) small_dx_as<T, ROUND, 2>(a, p, dz, lddz, w, n, out, s);
+  else if constexpr (sizeof(T) == 4 && !ROUND) small_dx_as<T, ROUND, 4>(a, p, dz, lddz, w, n, out, s);
+}
+void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
+  if (a.w_dtype == TK_BF16) small_dx_of<unsigned short, false>(a, p, dz, lddz, w, n, out, s);
+  else if (a.dtype == TK_BF16) small_dx_of<float, true>(a, p, dz, lddz, w, n, out, s);
+  else small_dx_of<float, false>(a, p, dz, lddz, w, n, out, s);
 }
 
-template <typename TX, typename TO>
+// Workgroups of 4 (bf16: 2) tiles of 16 vocabulary rows a wave where two a CU are left, else of one
+template <typename TX, typename TO, int RT>
 void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
-  const long blocks = ((n + 63) / 64) * dtf_cdiv(a.D, 16 * (16 / (int)sizeof(TX)));
-  hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx, static_cast<TO*>(out), a.N, a.D, n, rows, scale);
+  const long blocks = ((n + 64 * RT - 1) / (64 * RT)) * dtf_cdiv(a.D, 256 / (int)sizeof(TX));
+  if (RT > 1 && blocks < 512) return small_dw_as<TX, TO, 1>(a, dz, lddz, n, out, rows, scale, s);
+  hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO, RT>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx,
+                     static_cast<TO*>(out), a.N, a.D, n, rows, scale);
 }
 void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
-  if (a.dtype == TK_F32) small_dw_as<float, float>(a, dz, lddz, n, out, rows, scale, s);
-  else if (a.w_dtype == TK_F32) small_dw_as<unsigned short, float>(a, dz, lddz, n, out, rows, scale, s);
-  else small_dw_as<unsigned short, unsigned short>(a, dz, lddz, n, out, rows, scale, s);
+  if (a.dtype == TK_F32) small_dw_as<float, float, 4>(a, dz, lddz, n, out, rows, scale, s);
+  else if (a.w_dtype == TK_F32) small_dw_as<unsigned short, float, 2>(a, dz, lddz, n, out, rows, scale, s);
+  else small_dw_as<unsigned short, unsigned short, 2>(a, dz, lddz, n, out, rows, scale, s);
 }
 
 int check(const DtfVocabXentArgs* a) {

@@ -114,6 +114,31 @@ def test_sizes_of_the_large_blocks(n, v, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,wdtype,n,v,d", [
+    (torch.float32, torch.float32, 20, 33000, 9), (torch.float32, torch.float32, 33, 33000, 33), (torch.float32, torch.float32, 40, 33000, 300),
+    (torch.float32, torch.float32, 200, 8300, 130), (torch.float32, torch.float32, 255, 20001, 257), (torch.float32, torch.float32, 96, 16500, 64),
+    (torch.bfloat16, torch.bfloat16, 20, 33000, 700), (torch.bfloat16, torch.float32, 31, 33000, 701), (torch.float32, torch.float32, 700, 130, 1030)])
+def test_sizes_of_the_kernels_of_few_rows(dtype, wdtype, n, v, d):
+    """Sizes at which a workgroup takes one, two and four tiles of 16 rows; widths of whole and of broken 16-byte pieces."""
+    check(n, v, d, dtype, "cuda:0", wdtype=wdtype, bias=n % 2 == 0)
+
+
+@pytest.mark.gpu
+def test_a_weight_row_of_infinities_behind_a_broken_piece():
+    """Width 5: the 16-byte piece that ends a row reaches into the next one, whose logits are -inf here and stay apart."""
+    x, w, lab, b = draw(40, 300, 5, torch.float32, pad=0.0)
+    x, lab = x.abs() + 0.1, lab % 7
+    w[10::20] = -float("inf")
+    r, (dx, dw, db) = run(x, w, lab, b, "cuda:0")
+    keep = torch.ones(300, dtype=torch.bool)
+    keep[10::20] = False
+    want = exact(x, w[keep], lab, b[keep])
+    assert_within(r.loss_rows.cpu(), *want["rows"], "loss rows")
+    assert_within(dw.cpu()[keep], *want["dw"], "dweight")
+    assert not dw.cpu()[~keep].any() and not db.cpu()[~keep].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,wdtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
 def test_pieces_of_the_vocabulary(dtype, wdtype):
     """40 000 columns at 16 416 tokens are more than one piece (1 GiB of dz and dz^T), the last one ragged.  Column and row
