@@ -371,12 +371,21 @@ struct VxGemm : DtfGemmArgs {
   }
 };
 
+// The kernels of few rows.  Loads in their loops carry no conditions, which would keep the compiler from having several under
+// way: rows and steps past the last repeat it (their results are not stored, their products left out, or they meet zeros),
+// and waves whose pieces are all WHOLE have a loop of their own that does not look at the row's end.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ tk_u32x4 piece_of(const T* row, int c, int C) {
+  if constexpr (WHOLE) return *reinterpret_cast<const tk_u32x4_at2*>(row + c);
+  else return TkPiece<T, false>::load(row, c, C);
+}
+
 // Few rows, or few columns: 16 RT rows x 64 columns a workgroup, the four waves share K (64 bytes of a row a step, wave by
 // wave), operands straight from memory into the matrix instructions: one wave's 16 to 24 loads in flight, no staging, no
 // barrier in the loop.  Every row of W is read by ceil(M / 16 RT) workgroups, next to each other on one XCD.
 // Not ALIGNED (fp32 only): rows of any width, stride and alignment, the elements behind a row's end replaced by zeros.
 template <typename T, int EPI, int RT, bool ALIGNED>
-__global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
+__global__ __launch_bounds__(256, RT == 4 ? 2 : 1) void vx_skinny_kernel(VxGemm p) {
   typedef std::conditional_t<sizeof(T) == 4, float, unsigned short> E;
   constexpr int PER16 = Elem<T>::PER16, AHEAD = RT == 4 ? 2 : 4;
   __shared__ float s_acc[3][16 * RT][64];
@@ -406,30 +415,67 @@ __global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int steps = (p.K + 4 * PER16 - 1) / (4 * PER16);
-  for (int s = wave; s < steps; s += 4 * AHEAD) {
-    u32x4 a[AHEAD][RT], b[AHEAD][4];
+  // steps of 16 VEC elements: all of them if ALIGNED (pieces past the end are out of the buffer's range and read as zeros), else
+  // the whole ones, and the rest below
+  const int steps = ALIGNED ? (p.K + 4 * PER16 - 1) / (4 * PER16) : p.K / (4 * PER16);
+  struct Pieces { u32x4 a[AHEAD][RT], b[AHEAD][4]; };
+  auto load = [&](int s, Pieces& t) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int k = (s + 4 * u) * 4 + g;           // 16-byte piece of the row
-      const bool in = k * PER16 < p.K;
+      const int k = min(s + 4 * u, steps - 1) * 4 + g;       // 16-byte piece of the row
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        if constexpr (ALIGNED) a[u][i] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(in ? a_off[i] + k * 16u : kOOB), 0, 0);
-        else a[u][i] = in ? TkPiece<E, false>::load(a_row[i], k * PER16, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+        if constexpr (ALIGNED) t.a[u][i] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(k * PER16 < p.K ? a_off[i] + k * 16u : kOOB), 0, 0);
+        else t.a[u][i] = piece_of<true>(a_row[i], k * PER16, p.K);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (ALIGNED) b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(in ? b_off[j] + k * 16u : kOOB), 0, 0);
-        else b[u][j] = in ? TkPiece<E, false>::load(b_row[j], k * PER16, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+        if constexpr (ALIGNED) t.b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(k * PER16 < p.K ? b_off[j] + k * 16u : kOOB), 0, 0);
+        else t.b[u][j] = piece_of<true>(b_row[j], k * PER16, p.K);
       }
     }
+    if constexpr (RT == 4) __builtin_amdgcn_sched_barrier(0);
+  };
+  auto product = [&](int s, const Pieces& t) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
+    for (int u = 0; u < AHEAD; ++u) {
+      if (s + 4 * u >= steps) break;               // the same for the whole wave
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma_slot<T>(a[u][i], b[u][j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) mma_slot<T>(t.a[u][i], t.b[u][j], acc[i][j]);
+    }
+    if constexpr (RT == 4) __builtin_amdgcn_sched_barrier(0);
+  };
+  if (wave < steps) {
+    if constexpr (RT < 4) {                        // few products a load: four to seven waves a SIMD cover the latency
+      for (int s = wave; s < steps; s += 4 * AHEAD) {
+        Pieces t;
+        load(s, t);
+        product(s, t);
+      }
+    } else {                                       // two waves a SIMD: the next pieces are on their way during the products
+      Pieces t, next;
+      load(wave, t);
+      for (int s = wave; s < steps; s += 8 * AHEAD) {
+        load(s + 4 * AHEAD, next);
+        product(s, t);
+        load(s + 8 * AHEAD, t);
+        product(s + 4 * AHEAD, next);
+      }
+    }
+  }
+  if (!ALIGNED && wave == (steps & 3) && steps * 4 * PER16 < p.K) {
+    const int k = (steps * 4 + g) * PER16;
+    u32x4 a[RT], b[4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) a[i] = k < p.K ? piece_of<false>(a_row[i], k, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = k < p.K ? piece_of<false>(b_row[j], k, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma_slot<T>(a[i], b[j], acc[i][j]);
   }
   if (wave) {
 #pragma unroll
@@ -465,9 +511,10 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
   typedef TkPiece<T, false> P;
   constexpr int VEC = P::VEC;
   __shared__ float s_acc[3][4 * VEC * RT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int c = (int)blockIdx.x * 16 * VEC + VEC * fr, m0 = blockIdx.y * 16 * RT;
-  const long lo = (long)blockIdx.z * per, hi = min(n, lo + per);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
+  const int c = (int)blockIdx.x * 16 * VEC + VEC * fr, cc = c < D ? c : 0, m0 = blockIdx.y * 16 * RT;
+  // n is below 2^30; a wave's first 16 vocabulary rows of the range, and the last 16 it may reach
+  const int lo = (int)min((long)blockIdx.z * per, n), hi = (int)min(n, (long)lo + per), first = lo + 16 * wave, last = (hi - 1) & ~15;
   f32x4 acc[RT][VEC];
   const float* arow[RT];                         // rows past the last repeat it and are not stored
 #pragma unroll
@@ -476,30 +523,58 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
 #pragma unroll
     for (int q = 0; q < VEC; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  for (long v = lo + 16 * wave; v < hi; v += 128) {
-    f32x4 a[2][RT];
-    tk_u32x4 b[2][4];
+  constexpr int AHEAD = RT == 4 ? 1 : 2;
+  struct Pieces { f32x4 a[AHEAD][RT]; tk_u32x4 b[AHEAD][4]; };
+  auto run = [&](auto whole) {
+    auto load = [&](int v, Pieces& t) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const long at = v + 64 * u + 4 * g;        // dz is zero from n to its padded width, a multiple of 64 columns
+      for (int u = 0; u < AHEAD; ++u) {
+        const int at = min(v + 64 * u, last) + 4 * g;        // dz is zero from n to its padded width, a multiple of 64 columns
 #pragma unroll
-      for (int i = 0; i < RT; ++i) a[u][i] = v + 64 * u < hi ? *reinterpret_cast<const f32x4*>(arow[i] + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < RT; ++i) t.a[u][i] = *reinterpret_cast<const f32x4*>(arow[i] + at);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[u][j] = at + j < hi && c < D ? P::load(w + (at + j) * ldw, c, D) : tk_u32x4{0u, 0u, 0u, 0u};
-    }
+        for (int j = 0; j < 4; ++j) t.b[u][j] = piece_of<decltype(whole)::value>(w + (long)min(at + j, hi - 1) * ldw, cc, D);
+      }
+      __builtin_amdgcn_sched_barrier(0);         // all loads under way before the first product
+    };
+    auto product = [&](int v, const Pieces& t) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < AHEAD; ++u) {
+        if (v + 64 * u >= hi) break;             // the same for the whole wave
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float wv[VEC];
-        P::unpack(b[u][j], wv);
+        for (int j = 0; j < 4; ++j) {
+          float wv[VEC];
+          P::unpack(t.b[u][j], wv);
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          if (ROUND) wv[q] = tk_bf2f(tk_f2bf(wv[q]));
+          for (int q = 0; q < VEC; ++q) {
+            if (ROUND) wv[q] = tk_bf2f(tk_f2bf(wv[q]));
 #pragma unroll
-          for (int i = 0; i < RT; ++i) acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i][j], wv[q], acc[i][q], 0, 0, 0);
+            for (int i = 0; i < RT; ++i) acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.a[u][i][j], wv[q], acc[i][q], 0, 0, 0);
+          }
         }
       }
+      if constexpr (RT == 4) __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (RT < 4) {
+      for (int v = first; v < hi; v += 64 * AHEAD) {
+        Pieces t;
+        load(v, t);
+        product(v, t);
+      }
+    } else {                                     // the next pieces are on their way during the products
+      Pieces t, next;
+      load(first, t);
+      for (int v = first; v < hi; v += 128 * AHEAD) {
+        load(v + 64 * AHEAD, next);
+        product(v, t);
+        load(v + 128 * AHEAD, t);
+        product(v + 64 * AHEAD, next);
+      }
+    }
+  };
+  if (first < hi) {
+    if (__ballot(cc + VEC > D) == 0) run(std::true_type{});
+    else run(std::false_type{});
   }
   if (wave) {
 #pragma unroll
@@ -533,39 +608,52 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
 
 // dW: a wave owns 16 RT vocabulary rows and 16 VEC columns; the waves of a workgroup have the columns in common.
 template <typename TX, typename TO, int RT>
-__global__ __launch_bounds__(256) void vx_small_dw_kernel(const float* __restrict__ dz, long lddz, const TX* __restrict__ x, long ldx, TO* __restrict__ out,
-                                                          int M, int D, long n, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
+__global__ __launch_bounds__(256, RT > 1 ? 3 : 1) void vx_small_dw_kernel(const float* __restrict__ dz, long lddz, const TX* __restrict__ x, long ldx, TO* __restrict__ out,
+                                                          int M, int D, long n, int wide, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
   typedef TkPiece<TX, false> P;
   constexpr int VEC = P::VEC, OUT = 16 / sizeof(TO);
   const int lane = threadIdx.x & 63, fr = lane & 15, g = lane >> 4;
-  const int tiles = (D + 16 * VEC - 1) / (16 * VEC);
-  const long v0 = (long)(blockIdx.x / tiles) * 64 * RT + 16 * RT * (threadIdx.x >> 6);
-  const int c = (int)(blockIdx.x % tiles) * 16 * VEC + VEC * fr;
+  const int wave = threadIdx.x >> 6, across = wide ? 4 : 1, tiles = (D + 16 * VEC * across - 1) / (16 * VEC * across);
+  const long v0 = (long)(blockIdx.x / tiles) * (wide ? 16 * RT : 64 * RT) + (wide ? 0 : 16 * RT * wave);
+  const int c = ((int)(blockIdx.x % tiles) * across + (wide ? wave : 0)) * 16 * VEC + VEC * fr;
   f32x4 acc[RT][VEC];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int q = 0; q < VEC; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < M; k += 16) {
-    float a[4][RT];
-    tk_u32x4 b[4];
+  const int cc = c < D ? c : 0;
+  const float* col[RT];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = k + 4 * u + g;
+  for (int i = 0; i < RT; ++i) col[i] = dz + min(v0 + 16 * i + fr, n - 1);
+  auto run = [&](auto whole) {
+    for (int k = 0; k < M; k += 16) {
+      float a[4][RT], gr[4];
+      tk_u32x4 b[4];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) a[u][i] = row < M && v0 + 16 * i + fr < n ? dz[(long)row * lddz + v0 + 16 * i + fr] : 0.f;
-      b[u] = row < M && c < D && rows[row].g != 0.f ? P::load(x + (long)row * ldx, c, D) : tk_u32x4{0u, 0u, 0u, 0u};       // (see vx_transpose_kernel)
+      for (int u = 0; u < 4; ++u) {
+        const int row = min(k + 4 * u + g, M - 1);
+        gr[u] = rows[row].g;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) a[u][i] = col[i][(long)row * lddz];
+        b[u] = piece_of<decltype(whole)::value>(x + (long)row * ldx, cc, D);
+        if (k + 4 * u + g >= M) gr[u] = 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);         // all loads under way before the first product
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float xv[VEC];
+        P::unpack(b[u], xv);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          const float xq = gr[u] != 0.f ? xv[q] : 0.f;         // (see vx_transpose_kernel)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i], xq, acc[i][q], 0, 0, 0);
+        }
+      }
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float xv[VEC];
-      P::unpack(b[u], xv);
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i], xv[q], acc[i][q], 0, 0, 0);
-    }
-  }
+  };
+  if (__ballot(cc + VEC > D) == 0) run(std::true_type{});
+  else run(std::false_type{});
   const float f = *scale;
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -1103,10 +1191,11 @@ void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long 
 // Workgroups of 4 (bf16: 2) tiles of 16 vocabulary rows a wave where two a CU are left, else of one
 template <typename TX, typename TO, int RT>
 void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
-  const long blocks = ((n + 64 * RT - 1) / (64 * RT)) * dtf_cdiv(a.D, 256 / (int)sizeof(TX));
+  const int cols = 256 / (int)sizeof(TX), wide = a.D > 2 * cols;
+  const long blocks = wide ? ((n + 16 * RT - 1) / (16 * RT)) * dtf_cdiv(a.D, 4 * cols) : ((n + 64 * RT - 1) / (64 * RT)) * dtf_cdiv(a.D, cols);
   if (RT > 1 && blocks < 512) return small_dw_as<TX, TO, 1>(a, dz, lddz, n, out, rows, scale, s);
   hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO, RT>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx,
-                     static_cast<TO*>(out), a.N, a.D, n, rows, scale);
+                     static_cast<TO*>(out), a.N, a.D, n, wide, rows, scale);
 }
 void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
   if (a.dtype == TK_F32) small_dw_as<float, float, 4>(a, dz, lddz, n, out, rows, scale, s);
