@@ -385,11 +385,10 @@ __device__ __forceinline__ tk_u32x4 piece_of(const T* row, int c, int C) {
 // barrier in the loop.  Every row of W is read by ceil(M / 16 RT) workgroups, next to each other on one XCD.
 // Not ALIGNED (fp32 only): rows of any width, stride and alignment, the elements behind a row's end replaced by zeros.
 template <typename T, int EPI, int RT, bool ALIGNED>
-__global__ __launch_bounds__(256, RT == 4 ? 2 : 1) void vx_skinny_kernel(VxGemm p) {
+__global__ __launch_bounds__(256, RT < 4 ? 1 : ALIGNED ? 3 : 2) void vx_skinny_kernel(VxGemm p) {
   typedef std::conditional_t<sizeof(T) == 4, float, unsigned short> E;
-  constexpr int PER16 = Elem<T>::PER16, AHEAD = RT == 4 ? 2 : 4;
-  __shared__ float s_acc[3][16 * RT][64];
-  __shared__ __attribute__((aligned(16))) unsigned char s_out[2048 * RT];
+  constexpr int PER16 = Elem<T>::PER16, AHEAD = RT < 4 ? 4 : ALIGNED ? 1 : 2;
+  __shared__ __attribute__((aligned(16))) float s_acc[3][16 * RT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
   const int tiles_m = (p.M + 16 * RT - 1) / (16 * RT), wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
   const int m0 = (wg % tiles_m) * 16 * RT, n0 = (wg / tiles_m) * 64;
@@ -496,7 +495,8 @@ __global__ __launch_bounds__(256, RT == 4 ? 2 : 1) void vx_skinny_kernel(VxGemm 
         const int at = 16 * i + 4 * j + r;
         acc[i][j][r] = ((acc[i][j][r] + s_acc[0][at][lane]) + s_acc[1][at][lane]) + s_acc[2][at][lane];
       }
-  p.template epilogue<EPI, sizeof(T) == 4>(acc, s_out, m0, n0, lane);
+  // the epilogue's 2 KB a tile: memory that this wave, the only one left, has just read
+  p.template epilogue<EPI, sizeof(T) == 4>(acc, reinterpret_cast<unsigned char*>(s_acc), m0, n0, lane);
 }
 
 // The products of few rows (use_small), straight from X, W and the fp32 dz, with fp32 matrix instructions: the time goes
@@ -949,7 +949,7 @@ bool use_planes(int dtype, bool skinny) { return dtype == TK_F32 && !skinny; }
 // long as two workgroups a CU are left.
 int row_tiles(int dtype, long m, long others) {
   for (int rt = dtype == TK_BF16 ? 2 : 4; rt > 1; rt /= 2)
-    if (m > 8 * rt && (m + 16 * rt - 1) / (16 * rt) * others >= 512) return rt;
+    if (up(m, 16 * rt) <= up(m, 8 * rt) && (m + 16 * rt - 1) / (16 * rt) * others >= 512) return rt;
   return 1;
 }
 int skinny_tiles(int dtype, long m, long n) { return dtype == TK_BF16 ? 1 : row_tiles(dtype, m, (n + 63) / 64); }
