@@ -936,10 +936,12 @@ bool use_small(int dtype, long m) { return dtype == TK_BF16 ? m <= 32 : m < 256;
 
 // Logits by the kernel that shares K between the waves: where 128x128 blocks would leave most CUs idle or, with few rows, be
 // mostly empty (bf16: as long as W is small; a large one streams faster through the 128x128 blocks: 131072 x 4096, one row,
-// 203 against 227 us); fp32 with fewer rows than planes pay for always.
-bool use_skinny(int dtype, long m, long n) {
+// 203 against 227 us); fp32 with fewer rows than planes pay for always, and where the planes' 256x256 blocks would be too few (a
+// shallow K leaves most of the kernel's time to the epilogue, which one wave of four does here).
+bool use_skinny(int dtype, long m, long n, long k) {
   const long blocks = ((m + 127) / 128) * ((n + 127) / 128);
-  return blocks < 128 || (dtype == TK_F32 ? m < 256 : m <= 16 && blocks < 512);
+  if (dtype == TK_BF16) return blocks < 128 || (m <= 16 && blocks < 512);
+  return blocks < 128 || m < 256 || (k >= 256 && !use_pp(3, m, n, k, 1));
 }
 
 // fp32 logits from planes: they cost 10 bytes of traffic for every element of W, which pays from about 256 rows on.
@@ -1065,7 +1067,7 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.Vp = p.pieces == 1 ? a.V : std::min(vp, up((a.V + p.pieces - 1) / p.pieces, 256));
   p.pieces = (a.V + p.Vp - 1) / p.Vp;
   p.ldv = up(p.Vp, 64);
-  p.skinny = use_skinny(a.dtype, a.N, p.Vp);
+  p.skinny = use_skinny(a.dtype, a.N, p.Vp, a.D);
   p.direct = !use_planes(a.dtype, p.skinny);
   p.small = use_small(a.dtype, a.N);
   // copies: planes, or bf16 rows that are no whole aligned 16-byte pieces
