@@ -16,7 +16,9 @@
 // the same direction in every row.
 // Bound by the matrix cores, which the products keep 74-86 % busy: 8192 x 131072 x 4096 bf16 takes 25.1 ms forward and
 // backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of the
-// logits' launches are a third of their time.  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
+// logits' launches are a third of their time; 777 x 10007 x 512 fp32 0.36 ms.  Few rows are bound by reading W (bf16, 16 rows at
+// 65536 x 4096 forward and backward 0.56 ms: four passes over 0.54 GB), in fp32 from 32 rows on by its matrix rate (64 rows 1.43
+// ms: 96 TFLOP/s, a large library product 155).  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
 // type (bf16: half a step 2^-8 of each element, the same rounding that any bf16 product of dz has).
 //
 // fp32 operands are cut into three bf16 planes, x = x0 + x1 + x2 up to 2^-26 |x| (each plane takes eight more bits), and a
@@ -609,13 +611,13 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
 // dW: a wave owns 16 RT vocabulary rows and 16 VEC columns; the waves of a workgroup have the columns in common.
 template <typename TX, typename TO, int RT>
 __global__ __launch_bounds__(256, RT > 1 ? 3 : 1) void vx_small_dw_kernel(const float* __restrict__ dz, long lddz, const TX* __restrict__ x, long ldx, TO* __restrict__ out,
-                                                          int M, int D, long n, int wide, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
+                                                          int M, int D, long n, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
   typedef TkPiece<TX, false> P;
   constexpr int VEC = P::VEC, OUT = 16 / sizeof(TO);
   const int lane = threadIdx.x & 63, fr = lane & 15, g = lane >> 4;
-  const int wave = threadIdx.x >> 6, across = wide ? 4 : 1, tiles = (D + 16 * VEC * across - 1) / (16 * VEC * across);
-  const long v0 = (long)(blockIdx.x / tiles) * (wide ? 16 * RT : 64 * RT) + (wide ? 0 : 16 * RT * wave);
-  const int c = ((int)(blockIdx.x % tiles) * across + (wide ? wave : 0)) * 16 * VEC + VEC * fr;
+  const int tiles = (D + 16 * VEC - 1) / (16 * VEC);
+  const long v0 = (long)(blockIdx.x / tiles) * 64 * RT + 16 * RT * (threadIdx.x >> 6);
+  const int c = (int)(blockIdx.x % tiles) * 16 * VEC + VEC * fr;
   f32x4 acc[RT][VEC];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -931,30 +933,34 @@ bool use_pp(int planes, long m, long n, long k, int splits) {
   return m >= 256 && n >= 256 && k / splits >= 256 && blocks >= (deep >= 2048 ? 112 : 192);
 }
 
-// Up to so many rows the products read W and X as they are (vx_small_dx_kernel, vx_small_dw_kernel).
+// Up to so many rows the products read W and X as they are (vx_small_dx_kernel, vx_small_dw_kernel).  Forward and backward,
+// this way / through transposed copies and planes: bf16 at 65536 x 4096, 48 rows 0.86 / 0.87 ms, 64 rows 0.98 / 0.88; fp32 178
+// rows at 60668 x 1464 1.37 / 1.47 ms, 255 at 10000 x 2048 0.44 / 0.45, 300 at 30000 x 1024 0.80 / 0.81, 400 1.48 / 0.84.
 bool use_small(int dtype, long m) { return dtype == TK_BF16 ? m <= 32 : m < 256; }
 
 // Logits by the kernel that shares K between the waves: where 128x128 blocks would leave most CUs idle or, with few rows, be
 // mostly empty (bf16: as long as W is small; a large one streams faster through the 128x128 blocks: 131072 x 4096, one row,
 // 203 against 227 us); fp32 with fewer rows than planes pay for always, and where the planes' 256x256 blocks would be too few (a
-// shallow K leaves most of the kernel's time to the epilogue, which one wave of four does here).
+// shallow K leaves most of the kernel's time to the epilogue, which one wave of four does here): 1176 x 3000 x 300 forward and
+// backward 163 us, through planes 181.
 bool use_skinny(int dtype, long m, long n, long k) {
   const long blocks = ((m + 127) / 128) * ((n + 127) / 128);
   if (dtype == TK_BF16) return blocks < 128 || (m <= 16 && blocks < 512);
   return blocks < 128 || m < 256 || (k >= 256 && !use_pp(3, m, n, k, 1));
 }
 
-// fp32 logits from planes: they cost 10 bytes of traffic for every element of W, which pays from about 256 rows on.
+// fp32 logits from planes: where the kernel above does not take them.
 bool use_planes(int dtype, bool skinny) { return dtype == TK_F32 && !skinny; }
 
-// Tiles of 16 rows that one workgroup of the kernels of few rows takes (each element of W it reads serves all of them), as
-// long as two workgroups a CU are left.
+// Tiles of 16 rows that one workgroup of the fp32 kernels of few rows takes (each element of W it reads serves all of them):
+// as many as leave no more rows empty than half as many would, while two workgroups a CU are left.  One tile / this, at 65536 x
+// 4096, forward and backward: 32 rows 1.27 / 1.04 ms, 64 rows 2.17 / 1.43.  (bf16: two tiles at 32 rows made no difference.)
 int row_tiles(int dtype, long m, long others) {
-  for (int rt = dtype == TK_BF16 ? 2 : 4; rt > 1; rt /= 2)
+  for (int rt = dtype == TK_BF16 ? 1 : 4; rt > 1; rt /= 2)
     if (up(m, 16 * rt) <= up(m, 8 * rt) && (m + 16 * rt - 1) / (16 * rt) * others >= 512) return rt;
   return 1;
 }
-int skinny_tiles(int dtype, long m, long n) { return dtype == TK_BF16 ? 1 : row_tiles(dtype, m, (n + 63) / 64); }
+int skinny_tiles(int dtype, long m, long n) { return row_tiles(dtype, m, (n + 63) / 64); }
 
 // Rows of a wave's block in the logits' epilogue
 int wave_rows(const VxGemm& a, bool skinny) {
@@ -1180,9 +1186,12 @@ void small_dx_as(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, lo
 }
 template <typename T, bool ROUND>
 void small_dx_of(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
-  if (p.rt == 1) small_dx_as<T, ROUND, 1>(a, p, dz, lddz, w, n, out, s);
-  else if (p.rt == 2) small_dx_as<T, ROUND, 2>(a, p, dz, lddz, w, n, out, s);
-  else if constexpr (sizeof(T) == 4 && !ROUND) small_dx_as<T, ROUND, 4>(a, p, dz, lddz, w, n, out, s);
+  if constexpr (sizeof(T) == 4) {
+    if (p.rt == 2) return small_dx_as<T, ROUND, 2>(a, p, dz, lddz, w, n, out, s);
+    if constexpr (!ROUND)                        // bf16 activations: at most 32 rows
+      if (p.rt == 4) return small_dx_as<T, ROUND, 4>(a, p, dz, lddz, w, n, out, s);
+  }
+  small_dx_as<T, ROUND, 1>(a, p, dz, lddz, w, n, out, s);
 }
 void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
   if (a.w_dtype == TK_BF16) small_dx_of<unsigned short, false>(a, p, dz, lddz, w, n, out, s);
@@ -1193,11 +1202,10 @@ void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long 
 // Workgroups of 4 (bf16: 2) tiles of 16 vocabulary rows a wave where two a CU are left, else of one
 template <typename TX, typename TO, int RT>
 void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
-  const int cols = 256 / (int)sizeof(TX), wide = a.D > 2 * cols;
-  const long blocks = wide ? ((n + 16 * RT - 1) / (16 * RT)) * dtf_cdiv(a.D, 4 * cols) : ((n + 64 * RT - 1) / (64 * RT)) * dtf_cdiv(a.D, cols);
+  const long blocks = ((n + 64 * RT - 1) / (64 * RT)) * dtf_cdiv(a.D, 256 / (int)sizeof(TX));
   if (RT > 1 && blocks < 512) return small_dw_as<TX, TO, 1>(a, dz, lddz, n, out, rows, scale, s);
   hipLaunchKernelGGL((vx_small_dw_kernel<TX, TO, RT>), dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const TX*>(a.X), (long)a.ldx,
-                     static_cast<TO*>(out), a.N, a.D, n, wide, rows, scale);
+                     static_cast<TO*>(out), a.N, a.D, n, rows, scale);
 }
 void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
   if (a.dtype == TK_F32) small_dw_as<float, float, 4>(a, dz, lddz, n, out, rows, scale, s);
