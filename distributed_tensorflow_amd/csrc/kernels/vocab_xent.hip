@@ -1199,7 +1199,8 @@ void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long 
   else small_dx_of<float, false>(a, p, dz, lddz, w, n, out, s);
 }
 
-// Workgroups of 4 (bf16: 2) tiles of 16 vocabulary rows a wave where two a CU are left, else of one
+// Waves of 4 (bf16: 2) tiles of 16 vocabulary rows where two workgroups a CU are left, else of one.  One tile / this, at 65536 x
+// 4096, forward and backward: fp32 64 rows 1.51 / 1.43 ms, bf16 32 rows 0.70 / 0.66.
 template <typename TX, typename TO, int RT>
 void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
   const long blocks = ((n + 64 * RT - 1) / (64 * RT)) * dtf_cdiv(a.D, 256 / (int)sizeof(TX));
