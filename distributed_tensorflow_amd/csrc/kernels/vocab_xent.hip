@@ -673,6 +673,252 @@ __global__ __launch_bounds__(256, RT > 1 ? 3 : 1) void vx_small_dw_kernel(const 
     }
 }
 
+// The fp32 kernels of 17 rows and more: operands as they are in memory, cut into their three bf16 planes in registers, six
+// products of planes with the bf16 matrix instructions (96 cycles for 16 x 16 x 32 where fp32's take 256).  The next step's
+// loads are on their way during the products.
+struct VxSplit { bf16x8_t p[3]; };
+__device__ __forceinline__ VxSplit vx_split(const float (&v)[8]) {
+  VxSplit s;
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = v[e];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = tk_pack2(r[2 * e], r[2 * e + 1]);
+      r[2 * e] -= __uint_as_float(w[e] << 16);
+      r[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+    }
+    s.p[q] = __builtin_bit_cast(bf16x8_t, w);
+  }
+  return s;
+}
+template <int RT>
+__device__ __forceinline__ void vx_split_product(const VxSplit (&a)[RT], const VxSplit (&b)[4], f32x4 (&acc)[RT][4]) {
+  constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};        // the small products first
+#pragma unroll
+  for (int k = 0; k < 6; ++k)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i].p[PA[k]], b[j].p[PB[k]], acc[i][j], 0, 0, 0);
+}
+__device__ __forceinline__ void vx_eight(const tk_u32x4 (&q)[2], float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(q[e >> 2][e & 3]);
+}
+// The four waves' sums of a workgroup, in wave 0
+template <int RT>
+__device__ __forceinline__ void vx_join_waves(float (&s)[3][16 * RT][64], f32x4 (&acc)[RT][4], int wave, int lane) {
+  if (wave) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[wave - 1][16 * i + 4 * j + r][lane] = acc[i][j][r];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = 16 * i + 4 * j + r;
+        acc[i][j][r] = ((acc[i][j][r] + s[0][at][lane]) + s[1][at][lane]) + s[2][at][lane];
+      }
+}
+
+// Logits: 16 RT rows x 64 columns a workgroup, the waves take 32 elements of K each in turn (a lane 32 bytes of a row).
+template <int EPI, int RT>
+__global__ __launch_bounds__(256, 2) void vx_split_logits_kernel(VxGemm p) {
+  __shared__ __attribute__((aligned(16))) float s_acc[3][16 * RT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
+  const int tiles_m = (p.M + 16 * RT - 1) / (16 * RT), wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
+  const int m0 = (wg % tiles_m) * 16 * RT, n0 = (wg / tiles_m) * 64;
+  const float* a_row[RT];                        // rows and columns past the last repeat it: the epilogue leaves them out
+  const float* b_row[4];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) a_row[i] = static_cast<const float*>(p.A) + (long)min(m0 + 16 * i + fr, p.M - 1) * p.lda + 8 * g;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b_row[j] = static_cast<const float*>(p.B) + (long)min(n0 + 16 * j + fr, p.N - 1) * p.ldb + 8 * g;
+  f32x4 acc[RT][4];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = p.K >> 5;                    // whole ones; the rest below
+  tk_u32x4 a[RT][2], b[4][2];
+  auto load = [&](int s) {
+    const int k = min(s, steps - 1) * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j][h] = piece_of<true>(b_row[j], k + 4 * h, p.K);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[i][h] = piece_of<true>(a_row[i], k + 4 * h, p.K);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  VxSplit sa[RT], sb[4];
+  auto split = [&] {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { vx_eight(b[j], v); sb[j] = vx_split(v); }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) { vx_eight(a[i], v); sa[i] = vx_split(v); }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (wave < steps) {
+    load(wave);
+    for (int s = wave; s < steps; s += 4) {
+      split();
+      load(s + 4);
+      vx_split_product<RT>(sa, sb, acc);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (wave == (steps & 3) && steps * 32 < p.K) {
+    const int k = steps * 32, left = p.K - k - 8 * g;        // elements of this lane's eight that exist
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j][h] = 4 * h < left ? piece_of<false>(b_row[j] + k, 4 * h, left) : tk_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < RT; ++i) a[i][h] = 4 * h < left ? piece_of<false>(a_row[i] + k, 4 * h, left) : tk_u32x4{0u, 0u, 0u, 0u};
+    }
+    split();
+    vx_split_product<RT>(sa, sb, acc);
+  }
+  vx_join_waves<RT>(s_acc, acc, wave, lane);
+  if (wave) return;
+  // the epilogue's 2 KB a tile: memory that this wave, the only one left, has just read
+  p.template epilogue<EPI, true>(acc, reinterpret_cast<unsigned char*>(s_acc), m0, n0, lane);
+}
+
+// dX: workgroup (64 columns, 16 RT rows, range of the vocabulary); the waves take 32 vocabulary rows each in turn, a lane eight of
+// them and four columns.
+template <int RT>
+__global__ __launch_bounds__(256, 2) void vx_split_dx_kernel(const float* __restrict__ dz, long lddz, const float* __restrict__ w, long ldw, float* __restrict__ out,
+                                                             int M, int D, long n, int per, int ldo) {
+  __shared__ float s_acc[3][16 * RT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
+  const int c = (int)blockIdx.x * 64 + 4 * fr, cc = c < D ? c : 0, m0 = blockIdx.y * 16 * RT;
+  // n is below 2^30; a wave's first 32 vocabulary rows of the range, and the last 32 it may reach
+  const int lo = (int)min((long)blockIdx.z * per, n), hi = (int)min(n, (long)lo + per), first = lo + 32 * wave, last = (hi - 1) & ~31;
+  f32x4 acc[RT][4];
+  const float* arow[RT];                         // rows past the last repeat it and are not stored
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    arow[i] = dz + (long)min(m0 + 16 * i + fr, M - 1) * lddz;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto run = [&](auto whole) {
+    tk_u32x4 a[RT][2], b[8];
+    auto load = [&](int v) {
+      const int at = min(v, last) + 8 * g;       // dz is zero from n to its padded width, a multiple of 64 columns
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = piece_of<decltype(whole)::value>(w + (long)min(at + j, hi - 1) * ldw, cc, D);
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) a[i][h] = *reinterpret_cast<const tk_u32x4*>(arow[i] + at + 4 * h);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load(first);
+    for (int v = first; v < hi; v += 128) {
+      VxSplit sa[RT], sb[4];
+      float e[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = __uint_as_float(b[j][q]);
+        sb[q] = vx_split(e);
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) { vx_eight(a[i], e); sa[i] = vx_split(e); }
+      __builtin_amdgcn_sched_barrier(0);
+      load(v + 128);
+      vx_split_product<RT>(sa, sb, acc);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (first < hi) {
+    if (__ballot(cc + 4 > D) == 0) run(std::true_type{});
+    else run(std::false_type{});
+  }
+  vx_join_waves<RT>(s_acc, acc, wave, lane);
+  if (wave || c >= ldo) return;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = m0 + 16 * i + 4 * g + r;
+      if (row < M) *reinterpret_cast<f32x4*>(out + ((size_t)blockIdx.z * M + row) * ldo + c) = f32x4{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
+    }
+}
+
+// dW: a wave owns 64 vocabulary rows and 64 columns, 32 rows of X a step.
+__global__ __launch_bounds__(256, 2) void vx_split_dw_kernel(const float* __restrict__ dz, long lddz, const float* __restrict__ x, long ldx, float* __restrict__ out,
+                                                             int M, int D, long n, const VxRow* __restrict__ rows, const float* __restrict__ scale) {
+  const int lane = threadIdx.x & 63, fr = lane & 15, g = lane >> 4;
+  const int tiles = (D + 63) / 64;
+  const long v0 = (long)(blockIdx.x / tiles) * 256 + 64 * (threadIdx.x >> 6);
+  const int c = (int)(blockIdx.x % tiles) * 64 + 4 * fr, cc = c < D ? c : 0;
+  f32x4 acc[4][4];
+  const float* col[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    col[i] = dz + min(v0 + 16 * i + fr, n - 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto run = [&](auto whole) {
+    for (int k = 0; k < M; k += 32) {
+      float a[4][8], gr[8];
+      tk_u32x4 b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = min(k + 8 * g + j, M - 1);
+        gr[j] = rows[row].g;
+        b[j] = piece_of<decltype(whole)::value>(x + (long)row * ldx, cc, D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i][j] = col[i][(long)row * lddz];
+        if (k + 8 * g + j >= M) gr[j] = 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);         // all loads under way before the first product
+      VxSplit sa[4], sb[4];
+      float e[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = gr[j] != 0.f ? __uint_as_float(b[j][q]) : 0.f;      // (see vx_transpose_kernel)
+        sb[q] = vx_split(e);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sa[i] = vx_split(a[i]);
+      vx_split_product<4>(sa, sb, acc);
+    }
+  };
+  if (__ballot(cc + 4 > D) == 0) run(std::true_type{});
+  else run(std::false_type{});
+  const float f = *scale;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const long v = v0 + 16 * i + 4 * g + r;
+      if (v >= n || c >= D) continue;
+      const float t[4] = {acc[i][0][r] * f, acc[i][1][r] * f, acc[i][2][r] * f, acc[i][3][r] * f};
+      TkPiece<float, false>::store(out + v * D, c, D, t);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------- streaming helpers
 // dst[r, 0 .. ldd) = src[r, 0 .. cols) and zeros: an aligned, padded copy in the operands' type.
 template <typename TS, typename TD>
@@ -981,12 +1227,12 @@ void launch_gemm(const VxGemm& a, int splits, hipStream_t s) {
   }
 }
 
-template <int EPI, int RT>
+template <int EPI>
 void launch_skinny_f32(const VxGemm& a, hipStream_t s) {
-  const dim3 g((unsigned)(dtf_cdiv(a.M, 16 * RT) * dtf_cdiv(a.N, 64)));
+  const dim3 g((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64)));
   const bool aligned = a.K % 4 == 0 && a.lda % 4 == 0 && a.ldb % 4 == 0 && dtf_aligned16(a.A) && dtf_aligned16(a.B);
-  if (aligned) hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, RT, true>), g, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, RT, false>), g, dim3(256), 0, s, a);
+  if (aligned) hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, 1, true>), g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, 1, false>), g, dim3(256), 0, s, a);
 }
 template <int EPI>
 void launch_skinny(const VxGemm& a, hipStream_t s) {
@@ -994,11 +1240,11 @@ void launch_skinny(const VxGemm& a, hipStream_t s) {
     hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI, 1, true>), dim3((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64))), dim3(256), 0, s, a);
     return;
   }
-  switch (skinny_tiles(a.dtype, a.M, a.N)) {
-    case 1: launch_skinny_f32<EPI, 1>(a, s); break;
-    case 2: launch_skinny_f32<EPI, 2>(a, s); break;
-    default: launch_skinny_f32<EPI, 4>(a, s);
-  }
+  const int rt = skinny_tiles(a.dtype, a.M, a.N);
+  const dim3 g((unsigned)(dtf_cdiv(a.M, 16 * rt) * dtf_cdiv(a.N, 64)));
+  if (rt == 4) hipLaunchKernelGGL((vx_split_logits_kernel<EPI, 4>), g, dim3(256), 0, s, a);
+  else if (rt == 2) hipLaunchKernelGGL((vx_split_logits_kernel<EPI, 2>), g, dim3(256), 0, s, a);
+  else launch_skinny_f32<EPI>(a, s);
 }
 
 template <int EPI>
@@ -1188,15 +1434,20 @@ template <typename T, bool ROUND>
 void small_dx_of(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
   if constexpr (sizeof(T) == 4) {
     if (p.rt == 2) return small_dx_as<T, ROUND, 2>(a, p, dz, lddz, w, n, out, s);
-    if constexpr (!ROUND)                        // bf16 activations: at most 32 rows
-      if (p.rt == 4) return small_dx_as<T, ROUND, 4>(a, p, dz, lddz, w, n, out, s);
   }
   small_dx_as<T, ROUND, 1>(a, p, dz, lddz, w, n, out, s);
 }
 void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
   if (a.w_dtype == TK_BF16) small_dx_of<unsigned short, false>(a, p, dz, lddz, w, n, out, s);
   else if (a.dtype == TK_BF16) small_dx_of<float, true>(a, p, dz, lddz, w, n, out, s);
-  else small_dx_of<float, false>(a, p, dz, lddz, w, n, out, s);
+  else if (p.rt == 1) small_dx_of<float, false>(a, p, dz, lddz, w, n, out, s);
+  else {
+    const dim3 g((unsigned)dtf_cdiv(a.D, 64), (unsigned)dtf_cdiv(a.N, 16 * p.rt), (unsigned)p.sx);
+    const int per = (int)up((p.Vp + p.sx - 1) / p.sx, 64);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, dz, lddz, static_cast<const float*>(w), (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp); };
+    if (p.rt == 4) go(vx_split_dx_kernel<4>);
+    else go(vx_split_dx_kernel<2>);
+  }
 }
 
 // Waves of 4 (bf16: 2) tiles of 16 vocabulary rows where two workgroups a CU are left, else of one.  One tile / this, at 65536 x
@@ -1209,7 +1460,11 @@ void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, 
                      static_cast<TO*>(out), a.N, a.D, n, rows, scale);
 }
 void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
-  if (a.dtype == TK_F32) small_dw_as<float, float, 4>(a, dz, lddz, n, out, rows, scale, s);
+  const long blocks = ((n + 255) / 256) * dtf_cdiv(a.D, 64);
+  if (a.dtype == TK_F32 && a.N > 8 && blocks >= 512)
+    hipLaunchKernelGGL(vx_split_dw_kernel, dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const float*>(a.X), (long)a.ldx, static_cast<float*>(out), a.N, a.D,
+                       n, rows, scale);
+  else if (a.dtype == TK_F32) small_dw_as<float, float, 4>(a, dz, lddz, n, out, rows, scale, s);
   else if (a.w_dtype == TK_F32) small_dw_as<unsigned short, float, 2>(a, dz, lddz, n, out, rows, scale, s);
   else small_dw_as<unsigned short, unsigned short, 2>(a, dz, lddz, n, out, rows, scale, s);
 }
