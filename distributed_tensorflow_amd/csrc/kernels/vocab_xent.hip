@@ -17,8 +17,8 @@
 // Bound by the matrix cores, which the products keep 74-86 % busy: 8192 x 131072 x 4096 bf16 takes 25.1 ms forward and
 // backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of the
 // logits' launches are a third of their time; 777 x 10007 x 512 fp32 0.36 ms.  Few rows are bound by reading W (bf16, 16 rows at
-// 65536 x 4096 forward and backward 0.56 ms: four passes over 0.54 GB), in fp32 from 32 rows on by its matrix rate (64 rows 1.43
-// ms: 96 TFLOP/s, a large library product 155).  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
+// 65536 x 4096 forward and backward 0.56 ms: four passes over 0.54 GB), in fp32 from some 40 rows on by cutting and
+// multiplying planes (64 rows 1.25 ms: 110 TFLOP/s over the 8 N V D, a large fp32 library product 155).  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
 // type (bf16: half a step 2^-8 of each element, the same rounding that any bf16 product of dz has).
 //
 // fp32 operands are cut into three bf16 planes, x = x0 + x1 + x2 up to 2^-26 |x| (each plane takes eight more bits), and a
@@ -27,8 +27,8 @@
 // a sixteenth.  (Elements below 2^-110 lose their last planes: 10^-33 beside sums of order one.)
 //
 // Kernels: the 8-wave 256x256 GEMM (gemm_pingpong.h) where its blocks fill the chip, the 4-wave 128x128 one (gemm_tiled.h)
-// otherwise; logits of few rows or columns by a kernel that shares K between the waves; the products of few rows
-// by kernels that read W and write dW once, with fp32 matrix instructions, as have fp32 logits of under 256 rows.
+// otherwise; logits of few rows or columns by kernels that share K between the waves; the products of few rows by kernels that
+// read W and write dW once, with fp32 matrix instructions or, fp32 operands of 17 rows and more, planes cut in registers.
 // bf16 widths that are no multiple of 16 bytes, unaligned or strided operands go through zero-padded copies, piece by piece.
 #include <hip/hip_runtime.h>
 
@@ -382,109 +382,16 @@ __device__ __forceinline__ tk_u32x4 piece_of(const T* row, int c, int C) {
   else return TkPiece<T, false>::load(row, c, C);
 }
 
-// Few rows, or few columns: 16 RT rows x 64 columns a workgroup, the four waves share K (64 bytes of a row a step, wave by
-// wave), operands straight from memory into the matrix instructions: one wave's 16 to 24 loads in flight, no staging, no
-// barrier in the loop.  Every row of W is read by ceil(M / 16 RT) workgroups, next to each other on one XCD.
-// Not ALIGNED (fp32 only): rows of any width, stride and alignment, the elements behind a row's end replaced by zeros.
-template <typename T, int EPI, int RT, bool ALIGNED>
-__global__ __launch_bounds__(256, RT < 4 ? 1 : ALIGNED ? 3 : 2) void vx_skinny_kernel(VxGemm p) {
-  typedef std::conditional_t<sizeof(T) == 4, float, unsigned short> E;
-  constexpr int PER16 = Elem<T>::PER16, AHEAD = RT < 4 ? 4 : ALIGNED ? 1 : 2;
-  __shared__ __attribute__((aligned(16))) float s_acc[3][16 * RT][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
-  const int tiles_m = (p.M + 16 * RT - 1) / (16 * RT), wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
-  const int m0 = (wg % tiles_m) * 16 * RT, n0 = (wg / tiles_m) * 64;
-  const rsrc_t ra = make_rsrc(p.A, p.a_bytes), rb = make_rsrc(p.B, p.b_bytes);
-  // rows and columns past the last repeat it: the epilogue leaves them out
-  unsigned a_off[RT], b_off[4];
-  const E* a_row[RT];
-  const E* b_row[4];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int row = min(m0 + 16 * i + fr, p.M - 1);
-    a_off[i] = (unsigned)row * (unsigned)p.lda * (unsigned)sizeof(T);
-    a_row[i] = static_cast<const E*>(p.A) + (long)row * p.lda;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = min(n0 + 16 * j + fr, p.N - 1);
-    b_off[j] = (unsigned)row * (unsigned)p.ldb * (unsigned)sizeof(T);
-    b_row[j] = static_cast<const E*>(p.B) + (long)row * p.ldb;
-  }
-  f32x4 acc[RT][4];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // steps of 16 VEC elements: all of them if ALIGNED (pieces past the end are out of the buffer's range and read as zeros), else
-  // the whole ones, and the rest below
-  const int steps = ALIGNED ? (p.K + 4 * PER16 - 1) / (4 * PER16) : p.K / (4 * PER16);
-  struct Pieces { u32x4 a[AHEAD][RT], b[AHEAD][4]; };
-  auto load = [&](int s, Pieces& t) {
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int k = min(s + 4 * u, steps - 1) * 4 + g;       // 16-byte piece of the row
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if constexpr (ALIGNED) t.a[u][i] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(k * PER16 < p.K ? a_off[i] + k * 16u : kOOB), 0, 0);
-        else t.a[u][i] = piece_of<true>(a_row[i], k * PER16, p.K);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (ALIGNED) t.b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(k * PER16 < p.K ? b_off[j] + k * 16u : kOOB), 0, 0);
-        else t.b[u][j] = piece_of<true>(b_row[j], k * PER16, p.K);
-      }
-    }
-    if constexpr (RT == 4) __builtin_amdgcn_sched_barrier(0);
-  };
-  auto product = [&](int s, const Pieces& t) {
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      if (s + 4 * u >= steps) break;               // the same for the whole wave
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mma_slot<T>(t.a[u][i], t.b[u][j], acc[i][j]);
-    }
-    if constexpr (RT == 4) __builtin_amdgcn_sched_barrier(0);
-  };
-  if (wave < steps) {
-    if constexpr (RT < 4) {                        // few products a load: four to seven waves a SIMD cover the latency
-      for (int s = wave; s < steps; s += 4 * AHEAD) {
-        Pieces t;
-        load(s, t);
-        product(s, t);
-      }
-    } else {                                       // two waves a SIMD: the next pieces are on their way during the products
-      Pieces t, next;
-      load(wave, t);
-      for (int s = wave; s < steps; s += 8 * AHEAD) {
-        load(s + 4 * AHEAD, next);
-        product(s, t);
-        load(s + 8 * AHEAD, t);
-        product(s + 4 * AHEAD, next);
-      }
-    }
-  }
-  if (!ALIGNED && wave == (steps & 3) && steps * 4 * PER16 < p.K) {
-    const int k = (steps * 4 + g) * PER16;
-    u32x4 a[RT], b[4];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) a[i] = k < p.K ? piece_of<false>(a_row[i], k, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = k < p.K ? piece_of<false>(b_row[j], k, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mma_slot<T>(a[i], b[j], acc[i][j]);
-  }
+// The four waves' sums of a workgroup, in wave 0
+template <int RT>
+__device__ __forceinline__ void vx_join_waves(float (&s)[3][16 * RT][64], f32x4 (&acc)[RT][4], int wave, int lane) {
   if (wave) {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s_acc[wave - 1][16 * i + 4 * j + r][lane] = acc[i][j][r];
+        for (int r = 0; r < 4; ++r) s[wave - 1][16 * i + 4 * j + r][lane] = acc[i][j][r];
   }
   __syncthreads();
   if (wave) return;
@@ -495,13 +402,77 @@ __global__ __launch_bounds__(256, RT < 4 ? 1 : ALIGNED ? 3 : 2) void vx_skinny_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int at = 16 * i + 4 * j + r;
-        acc[i][j][r] = ((acc[i][j][r] + s_acc[0][at][lane]) + s_acc[1][at][lane]) + s_acc[2][at][lane];
+        acc[i][j][r] = ((acc[i][j][r] + s[0][at][lane]) + s[1][at][lane]) + s[2][at][lane];
       }
-  // the epilogue's 2 KB a tile: memory that this wave, the only one left, has just read
+}
+
+// Few rows, or few columns: 16 rows x 64 columns a workgroup, the four waves share K (64 bytes of a row a step, wave by wave),
+// operands straight from memory into the matrix instructions: one wave's 20 loads in flight, no staging, no barrier in the
+// loop.  Every row of W is read by ceil(M / 16) workgroups, next to each other on one XCD.
+// Not ALIGNED (fp32 only): rows of any width, stride and alignment, the elements behind a row's end replaced by zeros.
+template <typename T, int EPI, bool ALIGNED>
+__global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
+  typedef std::conditional_t<sizeof(T) == 4, float, unsigned short> E;
+  constexpr int PER16 = Elem<T>::PER16, AHEAD = 4;
+  __shared__ __attribute__((aligned(16))) float s_acc[3][16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
+  const int tiles_m = (p.M + 15) >> 4, wg = dtf_xcd_remap(blockIdx.x, gridDim.x);
+  const int m0 = (wg % tiles_m) * 16, n0 = (wg / tiles_m) * 64;
+  const rsrc_t ra = make_rsrc(p.A, p.a_bytes), rb = make_rsrc(p.B, p.b_bytes);
+  // rows and columns past the last repeat it: the epilogue leaves them out
+  const int row = min(m0 + fr, p.M - 1);
+  const unsigned a_off = (unsigned)row * (unsigned)p.lda * (unsigned)sizeof(T);
+  const E* const a_row = static_cast<const E*>(p.A) + (long)row * p.lda;
+  unsigned b_off[4];
+  const E* b_row[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int col = min(n0 + 16 * j + fr, p.N - 1);
+    b_off[j] = (unsigned)col * (unsigned)p.ldb * (unsigned)sizeof(T);
+    b_row[j] = static_cast<const E*>(p.B) + (long)col * p.ldb;
+  }
+  f32x4 acc[1][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // steps of 4 pieces of 16 bytes: all of them if ALIGNED (pieces past the end are out of the buffer's range and read as zeros),
+  // else the whole ones, and the rest below
+  const int steps = ALIGNED ? (p.K + 4 * PER16 - 1) / (4 * PER16) : p.K / (4 * PER16);
+  for (int s = wave; s < steps; s += 4 * AHEAD) {
+    u32x4 a[AHEAD], b[AHEAD][4];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = min(s + 4 * u, steps - 1) * 4 + g;       // 16-byte piece of the row
+      if constexpr (ALIGNED) {
+        const bool in = k * PER16 < p.K;
+        a[u] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(in ? a_off + k * 16u : kOOB), 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[u][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(in ? b_off[j] + k * 16u : kOOB), 0, 0);
+      } else {
+        a[u] = piece_of<true>(a_row, k * PER16, p.K);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[u][j] = piece_of<true>(b_row[j], k * PER16, p.K);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (s + 4 * u >= steps) break;               // the same for the whole wave
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma_slot<T>(a[u], b[u][j], acc[0][j]);
+    }
+  }
+  if (!ALIGNED && wave == (steps & 3) && steps * 4 * PER16 < p.K) {
+    const int k = (steps * 4 + g) * PER16;
+    const u32x4 a = k < p.K ? piece_of<false>(a_row, k, p.K) : tk_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mma_slot<T>(a, k < p.K ? piece_of<false>(b_row[j], k, p.K) : tk_u32x4{0u, 0u, 0u, 0u}, acc[0][j]);
+  }
+  vx_join_waves<1>(s_acc, acc, wave, lane);
+  if (wave) return;
+  // the epilogue's 2 KB: memory that this wave, the only one left, has just read
   p.template epilogue<EPI, sizeof(T) == 4>(acc, reinterpret_cast<unsigned char*>(s_acc), m0, n0, lane);
 }
 
-// The products of few rows (use_small), straight from X, W and the fp32 dz, with fp32 matrix instructions: the time goes
+// The products of few rows (few_rows), straight from X, W and the fp32 dz, with fp32 matrix instructions: the time goes
 // into reading W and writing dW once, so no transposed copies and no planes are made.  A lane's 16-byte piece of a row of W
 // (or X) is the operand of VEC instructions at once: instruction q takes column c0 + VEC fr + q.
 
@@ -525,7 +496,7 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
 #pragma unroll
     for (int q = 0; q < VEC; ++q) acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  constexpr int AHEAD = RT == 4 ? 1 : 2;
+  constexpr int AHEAD = 2;
   struct Pieces { f32x4 a[AHEAD][RT]; tk_u32x4 b[AHEAD][4]; };
   auto run = [&](auto whole) {
     auto load = [&](int v, Pieces& t) {
@@ -555,23 +526,11 @@ __global__ __launch_bounds__(256) void vx_small_dx_kernel(const float* __restric
           }
         }
       }
-      if constexpr (RT == 4) __builtin_amdgcn_sched_barrier(0);
     };
-    if constexpr (RT < 4) {
-      for (int v = first; v < hi; v += 64 * AHEAD) {
-        Pieces t;
-        load(v, t);
-        product(v, t);
-      }
-    } else {                                     // the next pieces are on their way during the products
-      Pieces t, next;
-      load(first, t);
-      for (int v = first; v < hi; v += 128 * AHEAD) {
-        load(v + 64 * AHEAD, next);
-        product(v, t);
-        load(v + 128 * AHEAD, t);
-        product(v + 64 * AHEAD, next);
-      }
+    for (int v = first; v < hi; v += 64 * AHEAD) {
+      Pieces t;
+      load(v, t);
+      product(v, t);
     }
   };
   if (first < hi) {
@@ -709,30 +668,6 @@ __device__ __forceinline__ void vx_eight(const tk_u32x4 (&q)[2], float (&v)[8]) 
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(q[e >> 2][e & 3]);
 }
-// The four waves' sums of a workgroup, in wave 0
-template <int RT>
-__device__ __forceinline__ void vx_join_waves(float (&s)[3][16 * RT][64], f32x4 (&acc)[RT][4], int wave, int lane) {
-  if (wave) {
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[wave - 1][16 * i + 4 * j + r][lane] = acc[i][j][r];
-  }
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 16 * i + 4 * j + r;
-        acc[i][j][r] = ((acc[i][j][r] + s[0][at][lane]) + s[1][at][lane]) + s[2][at][lane];
-      }
-}
-
 // Logits: 16 RT rows x 64 columns a workgroup, the waves take 32 elements of K each in turn (a lane 32 bytes of a row).
 template <int EPI, int RT>
 __global__ __launch_bounds__(256, 2) void vx_split_logits_kernel(VxGemm p) {
@@ -1179,31 +1114,31 @@ bool use_pp(int planes, long m, long n, long k, int splits) {
   return m >= 256 && n >= 256 && k / splits >= 256 && blocks >= (deep >= 2048 ? 112 : 192);
 }
 
-// Up to so many rows the products read W and X as they are (vx_small_dx_kernel, vx_small_dw_kernel).  Forward and backward,
-// this way / through transposed copies and planes: bf16 at 65536 x 4096, 48 rows 0.86 / 0.87 ms, 64 rows 0.98 / 0.88; fp32 178
-// rows at 60668 x 1464 1.37 / 1.47 ms, 255 at 10000 x 2048 0.44 / 0.45, 300 at 30000 x 1024 0.80 / 0.81, 400 1.48 / 0.84.
-bool use_small(int dtype, long m) { return dtype == TK_BF16 ? m <= 32 : m < 256; }
+// Up to so many rows the products read W and X as they are.  Forward and backward, this way / through transposed copies and
+// planes: bf16 at 65536 x 4096, 48 rows 0.86 / 0.87 ms, 64 rows 0.98 / 0.88; fp32 at 30000 x 1024, 256 rows 0.57 / 0.70 ms, 400
+// 0.83 / 0.84, 512 0.97 / 0.85; at 10000 x 512, 300 rows 185 / 209 us, 512 rows 245 / 258.
+bool few_rows(int dtype, long m) { return m <= (dtype == TK_BF16 ? 32 : 448); }
 
 // Logits by the kernel that shares K between the waves: where 128x128 blocks would leave most CUs idle or, with few rows, be
 // mostly empty (bf16: as long as W is small; a large one streams faster through the 128x128 blocks: 131072 x 4096, one row,
-// 203 against 227 us); fp32 with fewer rows than planes pay for always, and where the planes' 256x256 blocks would be too few (a
+// 203 against 227 us); fp32 with few rows always, and where the planes' 256x256 blocks would be too few (a
 // shallow K leaves most of the kernel's time to the epilogue, which one wave of four does here): 1176 x 3000 x 300 forward and
 // backward 163 us, through planes 181.
 bool use_skinny(int dtype, long m, long n, long k) {
   const long blocks = ((m + 127) / 128) * ((n + 127) / 128);
   if (dtype == TK_BF16) return blocks < 128 || (m <= 16 && blocks < 512);
-  return blocks < 128 || m < 256 || (k >= 256 && !use_pp(3, m, n, k, 1));
+  return blocks < 128 || few_rows(dtype, m) || (k >= 256 && !use_pp(3, m, n, k, 1));
 }
 
 // fp32 logits from planes: where the kernel above does not take them.
 bool use_planes(int dtype, bool skinny) { return dtype == TK_F32 && !skinny; }
 
-// Tiles of 16 rows that one workgroup of the fp32 kernels of few rows takes (each element of W it reads serves all of them):
-// as many as leave no more rows empty than half as many would, while two workgroups a CU are left.  One tile / this, at 65536 x
-// 4096, forward and backward: 32 rows 1.27 / 1.04 ms, 64 rows 2.17 / 1.43.  (bf16: two tiles at 32 rows made no difference.)
+// Tiles of 16 rows that one workgroup of the fp32 kernels of few rows takes (each element of W it reads and cuts serves all of
+// them), while two workgroups a CU are left.  Forward and backward: 64 rows at 65536 x 4096, one tile (fp32 instructions) 2.17 ms,
+// two 1.45, four 1.25; 140 rows at 30000 x 1024, two 0.53, four 0.41.  (bf16: two tiles at 32 rows made no difference.)
 int row_tiles(int dtype, long m, long others) {
   for (int rt = dtype == TK_BF16 ? 1 : 4; rt > 1; rt /= 2)
-    if (up(m, 16 * rt) <= up(m, 8 * rt) && (m + 16 * rt - 1) / (16 * rt) * others >= 512) return rt;
+    if (m > 8 * rt && (m + 16 * rt - 1) / (16 * rt) * others >= 512) return rt;
   return 1;
 }
 int skinny_tiles(int dtype, long m, long n) { return row_tiles(dtype, m, (n + 63) / 64); }
@@ -1231,13 +1166,13 @@ template <int EPI>
 void launch_skinny_f32(const VxGemm& a, hipStream_t s) {
   const dim3 g((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64)));
   const bool aligned = a.K % 4 == 0 && a.lda % 4 == 0 && a.ldb % 4 == 0 && dtf_aligned16(a.A) && dtf_aligned16(a.B);
-  if (aligned) hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, 1, true>), g, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, 1, false>), g, dim3(256), 0, s, a);
+  if (aligned) hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, true>), g, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((vx_skinny_kernel<unsigned int, EPI, false>), g, dim3(256), 0, s, a);
 }
 template <int EPI>
 void launch_skinny(const VxGemm& a, hipStream_t s) {
   if (a.dtype == TK_BF16) {
-    hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI, 1, true>), dim3((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((vx_skinny_kernel<unsigned short, EPI, true>), dim3((unsigned)(dtf_cdiv(a.M, 16) * dtf_cdiv(a.N, 64))), dim3(256), 0, s, a);
     return;
   }
   const int rt = skinny_tiles(a.dtype, a.M, a.N);
@@ -1321,7 +1256,7 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
   p.ldv = up(p.Vp, 64);
   p.skinny = use_skinny(a.dtype, a.N, p.Vp, a.D);
   p.direct = !use_planes(a.dtype, p.skinny);
-  p.small = use_small(a.dtype, a.N);
+  p.small = few_rows(a.dtype, a.N);
   // copies: planes, or bf16 rows that are no whole aligned 16-byte pieces
   const bool bf16 = a.dtype == TK_BF16;
   const bool odd_x = a.D % 8 || a.ldx % 8 || !dtf_aligned16(a.X), odd_w = a.D % 8 || a.ldw % 8 || !dtf_aligned16(a.W);
@@ -1430,24 +1365,15 @@ void small_dx_as(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, lo
   const int per = (int)up((p.Vp + p.sx - 1) / p.sx, 64);
   hipLaunchKernelGGL((vx_small_dx_kernel<T, ROUND, RT>), g, dim3(256), 0, s, dz, lddz, static_cast<const T*>(w), (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp);
 }
-template <typename T, bool ROUND>
-void small_dx_of(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
-  if constexpr (sizeof(T) == 4) {
-    if (p.rt == 2) return small_dx_as<T, ROUND, 2>(a, p, dz, lddz, w, n, out, s);
-  }
-  small_dx_as<T, ROUND, 1>(a, p, dz, lddz, w, n, out, s);
-}
 void small_dx(const DtfVocabXentArgs& a, const VxPlan& p, const float* dz, long lddz, const void* w, long n, float* out, hipStream_t s) {
-  if (a.w_dtype == TK_BF16) small_dx_of<unsigned short, false>(a, p, dz, lddz, w, n, out, s);
-  else if (a.dtype == TK_BF16) small_dx_of<float, true>(a, p, dz, lddz, w, n, out, s);
-  else if (p.rt == 1) small_dx_of<float, false>(a, p, dz, lddz, w, n, out, s);
-  else {
-    const dim3 g((unsigned)dtf_cdiv(a.D, 64), (unsigned)dtf_cdiv(a.N, 16 * p.rt), (unsigned)p.sx);
-    const int per = (int)up((p.Vp + p.sx - 1) / p.sx, 64);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, dz, lddz, static_cast<const float*>(w), (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp); };
-    if (p.rt == 4) go(vx_split_dx_kernel<4>);
-    else go(vx_split_dx_kernel<2>);
-  }
+  if (a.w_dtype == TK_BF16) return small_dx_as<unsigned short, false, 1>(a, p, dz, lddz, w, n, out, s);
+  if (a.dtype == TK_BF16) return p.rt == 1 ? small_dx_as<float, true, 1>(a, p, dz, lddz, w, n, out, s) : small_dx_as<float, true, 2>(a, p, dz, lddz, w, n, out, s);
+  if (p.rt == 1) return small_dx_as<float, false, 1>(a, p, dz, lddz, w, n, out, s);
+  const dim3 g((unsigned)dtf_cdiv(a.D, 64), (unsigned)dtf_cdiv(a.N, 16 * p.rt), (unsigned)p.sx);
+  const int per = (int)up((p.Vp + p.sx - 1) / p.sx, 64);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, dz, lddz, static_cast<const float*>(w), (long)a.ldw, out, a.N, a.D, n, per, (int)p.Dp); };
+  if (p.rt == 4) go(vx_split_dx_kernel<4>);
+  else go(vx_split_dx_kernel<2>);
 }
 
 // Waves of 4 (bf16: 2) tiles of 16 vocabulary rows where two workgroups a CU are left, else of one.  One tile / this, at 65536 x
@@ -1460,7 +1386,7 @@ void small_dw_as(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, 
                      static_cast<TO*>(out), a.N, a.D, n, rows, scale);
 }
 void small_dw(const DtfVocabXentArgs& a, const float* dz, long lddz, long n, void* out, const VxRow* rows, const float* scale, hipStream_t s) {
-  const long blocks = ((n + 255) / 256) * dtf_cdiv(a.D, 64);
+  const long blocks = ((n + 255) / 256) * dtf_cdiv(a.D, 64);              // (split_dw below 9 rows: half of its products are with rows that do not exist)
   if (a.dtype == TK_F32 && a.N > 8 && blocks >= 512)
     hipLaunchKernelGGL(vx_split_dw_kernel, dim3((unsigned)blocks), dim3(256), 0, s, dz, lddz, static_cast<const float*>(a.X), (long)a.ldx, static_cast<float*>(out), a.N, a.D,
                        n, rows, scale);

@@ -117,7 +117,9 @@ def test_sizes_of_the_large_blocks(n, v, d):
 @pytest.mark.parametrize("dtype,wdtype,n,v,d", [
     (torch.float32, torch.float32, 20, 33000, 9), (torch.float32, torch.float32, 33, 33000, 33), (torch.float32, torch.float32, 40, 33000, 300),
     (torch.float32, torch.float32, 200, 8300, 130), (torch.float32, torch.float32, 255, 20001, 257), (torch.float32, torch.float32, 96, 16500, 64),
-    (torch.bfloat16, torch.bfloat16, 20, 33000, 700), (torch.bfloat16, torch.float32, 31, 33000, 701), (torch.float32, torch.float32, 700, 130, 1030)])
+    (torch.bfloat16, torch.bfloat16, 20, 33000, 700), (torch.bfloat16, torch.float32, 31, 33000, 701), (torch.float32, torch.float32, 700, 130, 1030),
+    (torch.float32, torch.float32, 448, 6001, 95), (torch.float32, torch.float32, 449, 6001, 96), (torch.float32, torch.float32, 18, 33001, 31),
+    (torch.float32, torch.float32, 300, 17000, 32), (torch.float32, torch.float32, 6, 140000, 66)])
 def test_sizes_of_the_kernels_of_few_rows(dtype, wdtype, n, v, d):
     """Sizes at which a workgroup takes one, two and four tiles of 16 rows; widths of whole and of broken 16-byte pieces."""
     check(n, v, d, dtype, "cuda:0", wdtype=wdtype, bias=n % 2 == 0)
