@@ -411,7 +411,7 @@ __device__ __forceinline__ void vx_join_waves(float (&s)[3][16 * RT][64], f32x4 
 // loop.  Every row of W is read by ceil(M / 16) workgroups, next to each other on one XCD.
 // Not ALIGNED (fp32 only): rows of any width, stride and alignment, the elements behind a row's end replaced by zeros.
 template <typename T, int EPI, bool ALIGNED>
-__global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
+__global__ __launch_bounds__(256, 4) void vx_skinny_kernel(VxGemm p) {
   typedef std::conditional_t<sizeof(T) == 4, float, unsigned short> E;
   constexpr int PER16 = Elem<T>::PER16, AHEAD = 4;
   __shared__ __attribute__((aligned(16))) float s_acc[3][16][64];
@@ -453,6 +453,7 @@ __global__ __launch_bounds__(256) void vx_skinny_kernel(VxGemm p) {
         for (int j = 0; j < 4; ++j) b[u][j] = piece_of<true>(b_row[j], k * PER16, p.K);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);           // all loads under way before the first product
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (s + 4 * u >= steps) break;               // the same for the whole wave
