@@ -15,11 +15,12 @@
 // of dz is near -1 for every row that is not learned yet, and -1 is exact in bf16 where -1/count is off by up to 2^-8 in
 // the same direction in every row.
 // Bound by the matrix cores, which the products keep 74-86 % busy: 8192 x 131072 x 4096 bf16 takes 25.1 ms forward and
-// backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of the
-// logits' launches are a third of their time; 777 x 10007 x 512 fp32 0.36 ms.  Few rows are bound by reading W (bf16, 16 rows at
-// 65536 x 4096 forward and backward 0.56 ms: four passes over 0.54 GB), in fp32 from some 40 rows on by cutting and
-// multiplying planes (64 rows 1.25 ms: 110 TFLOP/s over the 8 N V D, a large fp32 library product 155).  Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands'
-// type (bf16: half a step 2^-8 of each element, the same rounding that any bf16 product of dz has).
+// backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of
+// the logits' launches are a third of their time; 777 x 10007 x 512 fp32 0.36 ms.  Few rows are bound by reading W (bf16, 16
+// rows at 65536 x 4096 forward and backward 0.56 ms: four passes over 0.54 GB), in fp32 from some 40 rows on by cutting and
+// multiplying planes (64 rows 1.21 ms: 113 TFLOP/s over the 8 N V D, a large fp32 library product 155).
+// Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands' type (bf16: half a step 2^-8 of
+// each element, the same rounding that any bf16 product of dz has).
 //
 // fp32 operands are cut into three bf16 planes, x = x0 + x1 + x2 up to 2^-26 |x| (each plane takes eight more bits), and a
 // product is the sum of the six plane products x0 w0, x0 w1, x1 w0, x0 w2, x2 w0, x1 w1, accumulated in fp32; what is left out
