@@ -126,6 +126,12 @@ def test_sizes_of_the_kernels_of_few_rows(dtype, wdtype, n, v, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,v,d", [(449, 9001, 33), (500, 16401, 130), (600, 16001, 520), (1000, 9001, 257), (1030, 700, 64)])
+def test_float32_sizes_of_the_planes(n, v, d):
+    check(n, v, d, torch.float32, "cuda:0", bias=n % 2 == 0)
+
+
+@pytest.mark.gpu
 def test_a_weight_row_of_infinities_behind_a_broken_piece():
     """Width 5: the 16-byte piece that ends a row reaches into the next one, whose logits are -inf here and stay apart."""
     x, w, lab, b = draw(40, 300, 5, torch.float32, pad=0.0)
@@ -240,7 +246,7 @@ def test_nan_stays_in_its_row(dev):
 
 @pytest.mark.parametrize("dev", devices())
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n,v", [(20, 100), (60, 300), (100, 300), (300, 16400)])
+@pytest.mark.parametrize("n,v", [(20, 100), (60, 300), (100, 300), (300, 16400), (70, 33000), (500, 8300)])
 def test_padding_rows_may_hold_nan_and_infinity(n, v, dtype, dev):
     """Every path of the backward pass: rows with the ignored label are as good as rows of zeros."""
     x, w, lab, b = draw(n, v, 40, dtype)
@@ -343,7 +349,7 @@ def test_refusals(dev):
 
 @pytest.mark.parametrize("dev", devices())
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n,v", [(20, 100), (100, 300), (300, 16400)])
+@pytest.mark.parametrize("n,v", [(20, 100), (100, 300), (300, 16400), (500, 8300)])
 def test_selected_gradients_are_those_of_a_full_call(n, v, dtype, dev):
     x, w, lab, b = (t.to(dev) for t in draw(n, v, 40, dtype))
     r = vx.vocab_xent_fwd(x, w, lab, b)
