@@ -37,7 +37,9 @@
 //     half a phase after the early group's, have returned (the compiler waits for them before the MFMAs that follow
 //     the next barrier) before any wave issues the overwriting load.
 //   * stages past the last K-tile (and chunks past K inside it) are issued with an out-of-range offset (the buffer
-//     range check delivers zeros), which keeps the counting uniform; vmcnt(0) before the epilogue: no load may land after the workgroup has ended.
+//     range check delivers zeros), which keeps the counting uniform.  They land in LDS all the same, some of them after the
+//     loop's last barrier, and the epilogue turns that LDS into scratch: every wave waits for its own (vmcnt(0)) and
+//     then passes one more barrier with all others.
 #pragma once
 #include "gemm_common.h"
 
@@ -209,8 +211,11 @@ __global__ __launch_bounds__(512) void gemm_pp_kernel(Args p) {
     PP_PHASE(PP_READ_A(1, REG_A1), 1, REG_A0, kt + 3, 1, 1, bq1, )
     PP_PHASE(, 1, REG_B0, kt + 3, 1, 0, bq0, )
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // nothing may land in LDS after this workgroup has ended
   if (wr == 0) __builtin_amdgcn_s_barrier();          // same number of barriers in both groups
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's stages of phases 5 to 8 (zeros) have landed ...
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();                       // ... and every other wave's, before any epilogue writes there
+  __builtin_amdgcn_sched_barrier(0);
 #undef PP_PHASE
 #undef PP_MMA
 #undef PP_BIAS
@@ -218,7 +223,7 @@ __global__ __launch_bounds__(512) void gemm_pp_kernel(Args p) {
 #undef PP_READ_B
 
   // ---- epilogue: acc[ha][i][hb][j][r] = C[m0 + wr*128 + ha*64 + 16i + 4g + r][n0 + wc*64 + hb*32 + 16j + fr]
-  // After the last barrier no wave reads operands any more, and every wave turns its own 16 KB of LDS into a
+  // After the last barrier no wave reads operands any more and no load is under way, and every wave turns its own 16 KB of LDS into a
   // transposition buffer for its 128x64 block: the MFMA result layout (a lane holds 4 rows of one column) would
   // otherwise store 2-byte pieces; from LDS every global store is 16 bytes per lane and whole 128/256-byte runs.
   typedef unsigned short T;
