@@ -11,9 +11,11 @@
 // dW = dz^T X (all products in the one form A[M,K] . B[N,K]^T of the tiled GEMMs).  The work is 8 N V D operations instead
 // of the 6 N V D of a program that stores the logits: at N = 8192, V = 131072 the fp32 logits would be 4 GB to write and
 // read again, 2.1 GB of bf16 dz per step go through a workspace of 1 GiB instead.
-// A factor that all rows share (1 / count, the gradient of a scalar loss) multiplies the sums, not dz: the label's element
-// of dz is near -1 for every row that is not learned yet, and -1 is exact in bf16 where -1/count is off by up to 2^-8 in
-// the same direction in every row.
+// What multiplies a whole row of dz (1 / count, the gradient of a scalar loss or of the row's own) stays out of dz where dz is
+// rounded to bf16: the label's element of dz is near -1 for every row that is not learned yet, and -1 is exact in bf16
+// where -1/count is off by up to 2^-8 in the same direction in every row.  The factor that the rows share multiplies the
+// sums (of gradients a row: the largest of them); what is left of a row's own, 1 where all are equal, multiplies its row of dX,
+// its share of db, and its X in the transposed copy that dW reads.
 // Bound by the matrix cores, which the products keep 74-86 % busy: 8192 x 131072 x 4096 bf16 takes 25.1 ms forward and
 // backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of
 // the logits' launches are a third of their time; 777 x 10007 x 512 fp32 0.36 ms.  Few rows are bound by reading W (bf16, 16
@@ -74,10 +76,11 @@ __device__ __forceinline__ void unrolled(F&& f) {
 
 // What the backward pass needs of a row: p = exp(z - top) / total, so dz = exp(z - top) scaled - [label] g with scaled = g /
 // total.  (exp(z - lse) would carry lse's own rounding, half a step of a value near 10, into every element of the row.)
+// dz in bf16: without g, scaled = 1 / total and 1 at the label.
 // Rows past the last and rows without a label have g = 0.
 struct alignas(16) VxRow {
   float top, scaled, g;
-  int label;                                     // -1 where the row has none
+  int label;                                     // -1 where the row has none, or no gradient
 };
 
 // exp(d) for d <= 0 or so with the rounding of d log2(e) made good: the product's error, up to |d| 2^-24 of the result, is
@@ -97,7 +100,7 @@ struct VxGemm : DtfGemmArgs {
   int v0;                                        // vocabulary index of column 0
   // VX_DZ (C = dz [M, ldc], Ct = dz^T [N, ldct], null: not needed; both leading dimensions are the padded widths, padding is
   // zeroed; of fp32 operands three bf16 planes each); VX_DZ32: C in fp32
-  const VxRow* rows;                             // padded to the block height
+  const VxRow* rows;                             // padded to the block height; VX_SUM: each row times its g, if given
   unsigned a_plane, b_plane;                     // bytes between the planes of the operands (EPI_PLANES)
   float* db_part;                                // [wave rows][N], optional
   // VX_SUM: fp32 result C32 [splits][M, ldc32] (accumulate: added to what is there), times *scale if given; with C the
@@ -226,18 +229,25 @@ struct VxGemm : DtfGemmArgs {
             const VxRow row = lrow[16 * ri + 4 * g + r];
             const int at = row.label - v0 - ccol - fr;
 #pragma unroll
-            for (int cj = 0; cj < 4; ++cj) acc[ri][cj][r] -= at == 16 * cj ? row.g : 0.f;
+            for (int cj = 0; cj < 4; ++cj) acc[ri][cj][r] -= at == 16 * cj ? (kExact ? row.g : 1.f) : 0.f;
           }
         }
       }
       if (db_part) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ri = 0; ri < RI; ++ri) {
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float own = kExact ? 1.f : lrow[16 * ri + 4 * g + r].g;
+#pragma unroll
+            for (int cj = 0; cj < 4; ++cj) sum[cj] += kExact ? acc[ri][cj][r] : acc[ri][cj][r] * own;
+          }
+        }
 #pragma unroll
         for (int cj = 0; cj < 4; ++cj) {
-          float v = 0.f;
-#pragma unroll
-          for (int ri = 0; ri < RI; ++ri)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v += acc[ri][cj][r];
+          float v = sum[cj];
           v += __shfl_xor(v, 16);
           v += __shfl_xor(v, 32);
           const int col = ccol + 16 * cj + fr;
@@ -363,8 +373,9 @@ struct VxGemm : DtfGemmArgs {
             for (int e = 0; e < 4; ++e) v[e] += o[e];
           }
           if (scale) {
+            const float own = rows ? f * rows[row].g : f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= f;
+            for (int e = 0; e < 4; ++e) v[e] *= own;
           }
           if (c16) *reinterpret_cast<uint2*>(&c16[(size_t)row * ldc + col]) = make_uint2(tk_pack2(v[0], v[1]), tk_pack2(v[2], v[3]));
           else *p = v;
@@ -868,8 +879,9 @@ __global__ __launch_bounds__(256) void vx_pack_kernel(const TS* __restrict__ src
 
 // dst[c, r] = src[r, c] for r < M, c < N; zeros for r in [M, ldt) and, of X (rows given), for rows without a gradient: in dW
 // they meet dz = 0, and a padding row that holds NaN or infinities must not make a sum of it.  64 x 64 tiles through LDS.
+// weighted: X times the row's g, rounded to bf16 (each element by its own half step at most, no direction in common).
 __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short* __restrict__ src, unsigned short* __restrict__ dst, int M, int N, long lds_, int ldt,
-                                                           const VxRow* __restrict__ rows) {
+                                                           const VxRow* __restrict__ rows, int weighted) {
   __shared__ unsigned short tile[64][72];
   const int across = (N + 63) >> 6, c0 = (int)(blockIdx.x % across) * 64, r0 = (int)(blockIdx.x / across) * 64;
 #pragma unroll
@@ -877,6 +889,14 @@ __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short*
     const int id = threadIdx.x + 256 * i, rr = id >> 3, ch = id & 7;
     u32x4 v = {0u, 0u, 0u, 0u};
     if (r0 + rr < M && c0 + ch * 8 < N && !(rows && rows[r0 + rr].g == 0.f)) v = *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + rr) * lds_ + c0 + ch * 8);
+    if (weighted && r0 + rr < M) {
+      const float own = rows[r0 + rr].g;
+      float f[8];
+      TkVec<unsigned short, 8>::unpack(v, f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= own;
+      v = TkVec<unsigned short, 8>::pack(f);
+    }
     *reinterpret_cast<u32x4*>(&tile[rr][ch * 8]) = v;
   }
   __syncthreads();
@@ -950,10 +970,10 @@ __global__ __launch_bounds__(256) void vx_planes_kernel(VxPlanes first, VxPlanes
   }
 }
 
-// out[r, c] = scale * sum of the splits' fp32 results, in their order, rounded to the output's type.
+// out[r, c] = scale [* the row's g] * sum of the splits' fp32 results, in their order, rounded to the output's type.
 template <typename T>
 __global__ __launch_bounds__(256) void vx_finish_kernel(const float* __restrict__ ws, int splits, int rows, int cols, int ldw, T* __restrict__ out, long ldo,
-                                                        const float* __restrict__ scale) {
+                                                        const float* __restrict__ scale, const VxRow* __restrict__ own) {
   const int quads = (cols + 3) >> 2;
   const long i = (long)blockIdx.x * 256 + threadIdx.x, row = i / quads;
   const int c = (int)(i - row * quads) * 4;
@@ -968,9 +988,10 @@ __global__ __launch_bounds__(256) void vx_finish_kernel(const float* __restrict_
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += s + u < splits ? o[u][e] : 0.f;
   }
+  const float f = own ? *scale * own[row].g : *scale;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (c + e < cols) tk_put(out + row * ldo + c + e, v[e] * *scale);
+    if (c + e < cols) tk_put(out + row * ldo + c + e, v[e] * f);
 }
 
 // db[c] = scale * sum of the wave rows' partial column sums
@@ -982,11 +1003,33 @@ __global__ __launch_bounds__(256) void vx_db_kernel(const float* __restrict__ pa
   db[c] = v * *scale;
 }
 
+__device__ __forceinline__ bool vx_has_label(long long lab, long long ignore, long V) { return lab != ignore && lab >= 0 && lab < V; }
+
+// *scale = the largest finite |dloss| of a row with a label, 1 if there is none but zeros.
+__global__ __launch_bounds__(1024) void vx_largest_kernel(const float* __restrict__ dloss, const long long* __restrict__ labels, int M, long V, long long ignore,
+                                                          float* __restrict__ scale) {
+  __shared__ float s[16];
+  float m = 0.f;
+  for (int r = threadIdx.x; r < M; r += 1024) {
+    const float v = fabsf(dloss[r]);
+    if (vx_has_label(labels[r], ignore, V) && v < __builtin_huge_valf()) m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) m = fmaxf(m, s[w]);
+  *scale = m > 0.f ? m : 1.f;
+}
+
+// apart (dz in bf16): g stays out of dz; of gradients a row it is relative to *scale, which vx_largest_kernel has left.
 __global__ __launch_bounds__(256) void vx_rows_kernel(const float* __restrict__ top, const float* __restrict__ total, const long long* __restrict__ labels, const float* __restrict__ dloss,
                                                       int dloss_rows, const long long* __restrict__ counts, int mean, int M, int Mp, long V,
-                                                      long long ignore, VxRow* __restrict__ rows, float* __restrict__ scale) {
+                                                      long long ignore, int apart, VxRow* __restrict__ rows, float* __restrict__ scale) {
   const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r == 0) {
+  if (r == 0 && !(apart && dloss_rows)) {
     const float up = dloss && !dloss_rows ? *dloss : 1.f;
     *scale = mean ? (counts[1] ? up / (float)counts[1] : 0.f) : up;
   }
@@ -994,11 +1037,11 @@ __global__ __launch_bounds__(256) void vx_rows_kernel(const float* __restrict__ 
   VxRow o = {0.f, 0.f, 0.f, -1};
   if (r < M) {
     const long long lab = labels[r];
-    if (lab != ignore && lab >= 0 && lab < V) {
+    if (vx_has_label(lab, ignore, V)) {
       o.top = top[r];
-      o.g = dloss_rows ? dloss[r] : 1.f;
-      o.scaled = o.g / total[r];
-      o.label = (int)lab;
+      o.g = !dloss_rows ? 1.f : apart ? dloss[r] / *scale : dloss[r];
+      o.scaled = (apart ? 1.f : o.g) / total[r];
+      if (o.g != 0.f) o.label = (int)lab;
     }
   }
   rows[r] = o;
@@ -1308,13 +1351,13 @@ VxPlan plan(const DtfVocabXentArgs& a, bool backward) {
 }
 
 template <typename T>
-void finish_as(const float* ws, int splits, long rows, int cols, int ldw, void* out, long ldo, const float* scale, hipStream_t s) {
+void finish_as(const float* ws, int splits, long rows, int cols, int ldw, void* out, long ldo, const float* scale, const VxRow* own, hipStream_t s) {
   const long n = rows * ((cols + 3) / 4);
-  hipLaunchKernelGGL((vx_finish_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, ws, splits, (int)rows, cols, ldw, static_cast<T*>(out), ldo, scale);
+  hipLaunchKernelGGL((vx_finish_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, ws, splits, (int)rows, cols, ldw, static_cast<T*>(out), ldo, scale, own);
 }
-void finish(const float* ws, int splits, long rows, int cols, int ldw, void* out, long ldo, int dtype, const float* scale, hipStream_t s) {
-  if (dtype == TK_BF16) finish_as<unsigned short>(ws, splits, rows, cols, ldw, out, ldo, scale, s);
-  else finish_as<float>(ws, splits, rows, cols, ldw, out, ldo, scale, s);
+void finish(const float* ws, int splits, long rows, int cols, int ldw, void* out, long ldo, int dtype, const float* scale, const VxRow* own, hipStream_t s) {
+  if (dtype == TK_BF16) finish_as<unsigned short>(ws, splits, rows, cols, ldw, out, ldo, scale, own, s);
+  else finish_as<float>(ws, splits, rows, cols, ldw, out, ldo, scale, own, s);
 }
 
 template <typename TS, typename TD>
@@ -1327,9 +1370,9 @@ void pack(const void* src, int sdt, void* dst, long rows, int cols, long lds_, l
   else pack_as<unsigned short, unsigned short>(src, dst, rows, cols, lds_, ldd, s);
 }
 
-void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, const VxRow* rows, hipStream_t s) {
+void transpose(const void* src, void* dst, long M, long N, long lds_, long ldt, const VxRow* rows, bool weighted, hipStream_t s) {
   const dim3 g((unsigned)(((N + 63) / 64) * ((ldt + 63) / 64)));            // one index: there may be more than 65535 tile rows
-  hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt, rows);
+  hipLaunchKernelGGL(vx_transpose_kernel, g, dim3(256), 0, s, static_cast<const unsigned short*>(src), static_cast<unsigned short*>(dst), (int)M, (int)N, lds_, (int)ldt, rows, (int)weighted);
 }
 
 VxPlanes planes_of(const void* src, void* dst, void* dst_t, long M, long N, long lds_, long Np, long Nt, long Mp, const VxRow* rows) {
@@ -1351,7 +1394,7 @@ Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int
   if (!p.direct || (p.planes == 3 && to_t)) planes = planes_of(src, p.direct ? nullptr : dst, to_t, rows, a.D, ld, p.ldd, p.Dp, ldt ? ldt : up(rows, 8), row_info);
   if (p.direct && copy) pack(src, from, dst, rows, a.D, ld, p.ldd, s);
   if (copy) o = {dst, p.ldd};
-  if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, row_info, s);
+  if (p.planes == 1 && to_t) transpose(o.p, to_t, rows, p.Dp, o.ld, ldt, row_info, row_info && a.dloss_rows, s);
   return o;
 }
 
@@ -1456,7 +1499,11 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
   VxRow* const rows = reinterpret_cast<VxRow*>(ws + p.rows);
   const int Mp = (int)up(a.N, 256);
   float* const scale = reinterpret_cast<float*>(rows + Mp);
-  hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.top, a.total, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, rows, scale);
+  const bool apart = p.planes == 1 && !p.small;  // dz is rounded to bf16
+  const VxRow* const own = apart && a.dloss_rows ? rows : nullptr;
+  if (own) hipLaunchKernelGGL(vx_largest_kernel, dim3(1), dim3(1024), 0, s, a.dloss, a.labels, a.N, a.V, a.ignore, scale);
+  hipLaunchKernelGGL(vx_rows_kernel, dim3(Mp / 256), dim3(256), 0, s, a.top, a.total, a.labels, a.dloss, a.dloss_rows, a.counts, a.mean, a.N, Mp, a.V, a.ignore, (int)apart,
+                     rows, scale);
   VxPlanes of_x = {}, of_w = {};
   const Operand X = prepare(a, p, a.X, a.dtype, a.N, a.ldx, p.pack_x, ws + p.x, a.dW && !p.small ? ws + p.xt : nullptr, p.ldn, rows, of_x, s);
   const int large = p.direct ? 1 : p.planes;     // planes of the logits' operands
@@ -1496,6 +1543,7 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
       d.accumulate = v0 > 0;                     // the last, shorter piece adds to its first splits only
       if (p.direct_dx && v0 + n == a.V) {
         d.scale = scale;
+        d.rows = own;
         if (a.dtype == TK_BF16) d.C = a.dX;
         d.ldc = a.D;
       }
@@ -1513,9 +1561,9 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
         d.ldc = a.D;
       }
       launch_gemm<VX_SUM>(d, p.sw, s);
-      if (!p.direct_dw) finish(dw32, p.sw, n, a.D, (int)p.Dp, out, a.D, a.w_dtype, scale, s);
+      if (!p.direct_dw) finish(dw32, p.sw, n, a.D, (int)p.Dp, out, a.D, a.w_dtype, scale, nullptr, s);
     }
   }
-  if (a.dX && !p.direct_dx) finish(dx32, p.small ? (int)p.pieces * p.sx : p.sx, a.N, a.D, (int)p.Dp, a.dX, a.D, a.dtype, scale, s);
+  if (a.dX && !p.direct_dx) finish(dx32, p.small ? (int)p.pieces * p.sx : p.sx, a.N, a.D, (int)p.Dp, a.dX, a.D, a.dtype, scale, own, s);
   return dtf_check_launch();
 }
