@@ -27,7 +27,13 @@
 // fp32 operands are cut into three bf16 planes, x = x0 + x1 + x2 up to 2^-26 |x| (each plane takes eight more bits), and a
 // product is the sum of the six plane products x0 w0, x0 w1, x1 w0, x0 w2, x2 w0, x1 w1, accumulated in fp32; what is left out
 // is below 2^-25 of |x w|, under an fp32 rounding.  Six bf16 matrix products cost less than one in fp32, whose matrix rate is
-// a sixteenth.  (Elements below 2^-110 lose their last planes: 10^-33 beside sums of order one.)
+// a sixteenth.  (Elements below 2^-110 lose their last planes: 10^-33 beside sums of order one.)  An infinity has no planes
+// that a sum of six products could be made of (0 or a remainder of the other sign times infinity is NaN), and a finite
+// number may round to one in its first plane: whoever finds infinities or NaN in its sums makes them again from the
+// operands as they are, with fp32 instructions, and takes those that were not finite from there (the others keep their
+// bits: what a neighbouring row holds does not matter).  Finite operands pay one instruction for every element of the result.
+// The large products dX and dW of planes cut beforehand do not: an infinity that meets a dz other than 0 (its row's loss is
+// infinite then) gives NaN.
 //
 // Kernels: the 8-wave 256x256 GEMM (gemm_pingpong.h) where its blocks fill the chip, the 4-wave 128x128 one (gemm_tiled.h)
 // otherwise; logits of few rows or columns by kernels that share K between the waves; the products of few rows by kernels that
@@ -92,6 +98,32 @@ __device__ __forceinline__ float exp_exact(float d) {
   return fmaf(e * 0.693147181f, lo, e);
 }
 
+template <bool WHOLE, typename T>
+__device__ __forceinline__ tk_u32x4 piece_of(const T* row, int c, int C) {
+  if constexpr (WHOLE) return *reinterpret_cast<const tk_u32x4_at2*>(row + c);
+  else return TkPiece<T, false>::load(row, c, C);
+}
+
+// Whether one of the wave's sums is infinite or NaN, and such sums taken from t
+template <int I, int J>
+__device__ __forceinline__ bool vx_not_finite(const f32x4 (&acc)[I][J]) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t = fmaf(acc[i][j][r], 0.f, t);
+  return __ballot(t != t) != 0;
+}
+template <int J>
+__device__ __forceinline__ void vx_mend(f32x4 (&acc)[J], const f32x4 (&t)[J]) {
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[j][r] = fabsf(acc[j][r]) < __builtin_huge_valf() ? acc[j][r] : t[j][r];
+}
+
 struct VxGemm : DtfGemmArgs {
   // VX_LSE
   const long long* labels;
@@ -102,6 +134,10 @@ struct VxGemm : DtfGemmArgs {
   // zeroed; of fp32 operands three bf16 planes each); VX_DZ32: C in fp32
   const VxRow* rows;                             // padded to the block height; VX_SUM: each row times its g, if given
   unsigned a_plane, b_plane;                     // bytes between the planes of the operands (EPI_PLANES)
+  // fp32 logits made of planes: the operands as they are ([M, D] and [N, D]); null: not made of planes
+  const float* x32; const float* w32;
+  long ldx32, ldw32;
+  int D;
   float* db_part;                                // [wave rows][N], optional
   // VX_SUM: fp32 result C32 [splits][M, ldc32] (accumulate: added to what is there), times *scale if given; with C the
   // sum goes there as bf16 [M, ldc] instead
@@ -138,6 +174,13 @@ struct VxGemm : DtfGemmArgs {
     }
     constexpr bool kExact = F32 || EPI == VX_DZ32;
     const float NEG_INF = -__builtin_huge_valf();
+    if constexpr (F32) {
+#pragma unroll
+      for (int ri = 0; ri < RI; ++ri)            // one home for them on both ways: else a second set of accumulators is kept
+#pragma unroll
+        for (int cj = 0; cj < 4; ++cj) asm volatile("" : "+v"(acc[ri][cj]));
+      if (x32 && vx_not_finite(acc)) again<RI>(acc, crow, ccol, lane);
+    }
     if (bias) {
 #pragma unroll
       for (int cj = 0; cj < 4; ++cj) {
@@ -280,6 +323,42 @@ struct VxGemm : DtfGemmArgs {
     }
   }
 
+  // The block's sums again, with fp32 instructions: a lane's 16-byte piece of a row is the operand of four.  Rows and columns
+  // past the last repeat it.  Two tiles of 16 rows at a time: all of them would cost the kernel a wave's registers.
+  template <int RI>
+  __device__ __forceinline__ void again(f32x4 (&acc)[RI][4], int crow, int ccol, int lane) const {
+    constexpr int H = RI > 1 ? 2 : 1;
+    const int fr = lane & 15, g = lane >> 4;
+    const float* b_row[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b_row[j] = w32 + (long)min(ccol + 16 * j + fr, N - 1) * ldw32;
+    unrolled<0, RI / H>([&](auto Half) {
+      constexpr int i0 = Half * H;
+      f32x4 t[H][4];
+#pragma unroll
+      for (int i = 0; i < H; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int k0 = 0; k0 < D; k0 += 16) {
+        tk_u32x4 b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = piece_of<false>(b_row[j], k0 + 4 * g, D);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          const tk_u32x4 a = piece_of<false>(x32 + (long)min(crow + 16 * (i0 + i) + fr, M - 1) * ldx32, k0 + 4 * g, D);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              t[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[j][e]), t[i][j], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < H; ++i) vx_mend(acc[i0 + i], t[i]);
+    });
+  }
+
   // Both images are turned in LDS, so that every global store is 16 bytes a lane.
   template <int RI, bool PLANES>
   __device__ __forceinline__ void store_dz(f32x4 (&acc)[RI][4], unsigned char* wl, int crow, int ccol, int lane, int plane) const {
@@ -388,12 +467,6 @@ struct VxGemm : DtfGemmArgs {
 // The kernels of few rows.  Loads in their loops carry no conditions, which would keep the compiler from having several under
 // way: rows and steps past the last repeat it (their results are not stored, their products left out, or they meet zeros),
 // and waves whose pieces are all WHOLE have a loop of their own that does not look at the row's end.
-template <bool WHOLE, typename T>
-__device__ __forceinline__ tk_u32x4 piece_of(const T* row, int c, int C) {
-  if constexpr (WHOLE) return *reinterpret_cast<const tk_u32x4_at2*>(row + c);
-  else return TkPiece<T, false>::load(row, c, C);
-}
-
 // The four waves' sums of a workgroup, in wave 0
 template <int RT>
 __device__ __forceinline__ void vx_join_waves(float (&s)[3][16 * RT][64], f32x4 (&acc)[RT][4], int wave, int lane) {
@@ -800,6 +873,23 @@ __global__ __launch_bounds__(256, 2) void vx_split_dx_kernel(const float* __rest
     if (__ballot(cc + 4 > D) == 0) run(std::true_type{});
     else run(std::false_type{});
   }
+  if (vx_not_finite(acc))                        // (see the head of this file)
+    unrolled<0, RT>([&](auto I) {
+      f32x4 t[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int v = first; v < hi; v += 128)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int at = v + 8 * g + j;
+          const float e = arow[I][at];
+          const tk_u32x4 b = piece_of<false>(w + (long)min(at, hi - 1) * ldw, cc, D);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) t[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(e, __uint_as_float(b[q]), t[q], 0, 0, 0);
+        }
+      vx_mend(acc[I], t);
+    });
   vx_join_waves<RT>(s_acc, acc, wave, lane);
   if (wave || c >= ldo) return;
 #pragma unroll
@@ -855,6 +945,22 @@ __global__ __launch_bounds__(256, 2) void vx_split_dw_kernel(const float* __rest
   };
   if (__ballot(cc + 4 > D) == 0) run(std::true_type{});
   else run(std::false_type{});
+  if (vx_not_finite(acc))                        // (see the head of this file)
+    unrolled<0, 4>([&](auto I) {
+      f32x4 t[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int k = 0; k < M; k += 4) {
+        const int row = min(k + g, M - 1);
+        const bool in = k + g < M && rows[row].g != 0.f;
+        const float e = k + g < M ? col[I][(long)row * lddz] : 0.f;
+        const tk_u32x4 b = piece_of<false>(x + (long)row * ldx, cc, D);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(e, in ? __uint_as_float(b[q]) : 0.f, t[q], 0, 0, 0);
+      }
+      vx_mend(acc[I], t);
+    });
   const float f = *scale;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -911,6 +1017,12 @@ __global__ __launch_bounds__(256) void vx_transpose_kernel(const unsigned short*
   }
 }
 
+// Nearest bf16, but the largest finite one for finite numbers beyond it: 0 times such an element stays 0.
+__device__ __forceinline__ unsigned short vx_first_plane(float v) {
+  const unsigned short q = tk_f2bf(v);
+  return (q & 0x7fff) == 0x7f80 && fabsf(v) < __builtin_huge_valf() ? q - 1 : q;
+}
+
 // The three bf16 planes of an fp32 matrix [M, N] (any stride and alignment), straight [3][M, Np] and / or transposed
 // [3][Nt, Mp], zeros in the padding; in the transposed one also for rows without a gradient (see vx_transpose_kernel).
 // Two matrices a launch: those of a small X are latency only, beside W's they cost nothing.
@@ -957,7 +1069,7 @@ __global__ __launch_bounds__(256) void vx_planes_kernel(VxPlanes first, VxPlanes
           unsigned e[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const unsigned short lo = tk_f2bf(v[2 * k]), hi = tk_f2bf(v[2 * k + 1]);
+            const unsigned short lo = vx_first_plane(v[2 * k]), hi = vx_first_plane(v[2 * k + 1]);
             e[k] = (unsigned)lo | ((unsigned)hi << 16);
             const float dl = v[2 * k] - tk_bf2f(lo), dh = v[2 * k + 1] - tk_bf2f(hi);
             v[2 * k] = fabsf(dl) < __builtin_huge_valf() ? dl : 0.f;
@@ -1398,6 +1510,16 @@ Operand prepare(const DtfVocabXentArgs& a, const VxPlan& p, const void* src, int
   return o;
 }
 
+// fp32 logits that are made of planes, cut beforehand or in registers
+void operands_as_they_are(VxGemm& g, const DtfVocabXentArgs& a, long v0, const VxPlan& p) {
+  if (a.dtype != TK_F32 || (p.skinny && skinny_tiles(a.dtype, g.M, g.N) == 1)) return;
+  g.x32 = static_cast<const float*>(a.X);
+  g.w32 = static_cast<const float*>(a.W) + v0 * a.ldw;
+  g.ldx32 = a.ldx;
+  g.ldw32 = a.ldw;
+  g.D = a.D;
+}
+
 // dz in fp32 for the kernels of few rows
 void launch_small_dz(const VxGemm& a, bool skinny, hipStream_t s) {
   if (skinny) launch_skinny<VX_DZ32>(a, s);
@@ -1478,6 +1600,7 @@ DTF_EXPORT int dtf_vocab_xent_fwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     g.part = reinterpret_cast<float2*>(ws + p.part);
     g.target = reinterpret_cast<float2*>(ws + p.target);
     g.v0 = (int)v0;
+    operands_as_they_are(g, a, v0, p);
     launch_logits<VX_LSE>(g, p.skinny, s);
   }
   VxJoin j = {reinterpret_cast<const float2*>(ws + p.part), reinterpret_cast<const float2*>(ws + p.target), a.labels, a.lse, a.top, a.total, a.loss_rows, a.loss,
@@ -1516,6 +1639,7 @@ DTF_EXPORT int dtf_vocab_xent_bwd(const DtfVocabXentArgs* ap, hipStream_t s) {
     launch_planes(of_x, of_w, s);
     VxGemm g = operands(X.p, W.p, a.dtype, large, a.N, (int)n, p.K, X.ld, W.ld);
     g.bias = a.bias ? a.bias + v0 : nullptr;
+    operands_as_they_are(g, a, v0, p);
     g.rows = rows;
     g.v0 = (int)v0;
     g.C = p.small ? ws + p.dz32 : a.dX ? ws + p.dz : nullptr;
