@@ -10,11 +10,16 @@ the other branch of a residual block in the same pass.
 tensor on x's device, whose value the kernel reads when it runs.  A captured graph that advances such a counter draws a
 new mask in every replay; the backward pass uses the value that its forward pass saw.
 
+Under activation checkpointing a forward pass runs twice.  ``FusedDropout`` then draws the first one's mask again (it knows
+the call by a number from PyTorch's CPU generator, whose state ``torch.utils.checkpoint`` restores).  ``dropout`` is a
+function: give the checkpointed part a ``step`` that has not moved on in between.
+
 The reference has no dropout; the generator is the one of the truncated-normal initialiser (distributed.py:67-72).
 """
 from __future__ import annotations
 
 import ctypes as C
+from collections import OrderedDict
 from typing import Optional, Union
 
 import torch
@@ -25,6 +30,7 @@ from . import _lib, reference
 from ._token import dtype_code, launch, same_device
 
 _protos_done = False
+REMEMBERED = 1024          # calls of a FusedDropout whose step is kept for a recomputation
 
 
 def _kernels():
@@ -73,10 +79,11 @@ def dropout_apply(x: torch.Tensor, rate: float, seed: int, step: Union[int, torc
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, rate, seed, step):
-        used = step
+    def forward(ctx, x, residual, rate, seed, step, used):
         if isinstance(step, torch.Tensor):                 # the counter may have moved on when backward() runs
-            used = torch.empty(1, dtype=torch.int64, device=x.device)
+            used = torch.empty(1, dtype=torch.int64, device=x.device) if used is None else used
+        else:
+            used = step
         y = dropout_apply(x, rate, seed, step, residual, used if used is not step else None)
         ctx.rate, ctx.seed, ctx.has_res = rate, seed, residual is not None
         ctx.step = used
@@ -86,7 +93,13 @@ class _Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         dx = dropout_apply(dy, ctx.rate, ctx.seed, ctx.step) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.has_res else None, None, None, None
+        return dx, dy if ctx.has_res else None, None, None, None, None
+
+
+def _dropout(x, rate, seed, step, residual, used=None):
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, rate, seed, step, used)
+    return dropout_apply(x, rate, seed, step, residual, used)
 
 
 def dropout(x: torch.Tensor, rate: float, seed: int, step: Union[int, torch.Tensor] = 0,
@@ -94,14 +107,17 @@ def dropout(x: torch.Tensor, rate: float, seed: int, step: Union[int, torch.Tens
     """``[residual +] dropout(x)``; without ``training`` nothing is dropped."""
     if not training:
         return x if residual is None else x + residual
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, rate, seed, step)
-    return dropout_apply(x, rate, seed, step, residual)
+    return _dropout(x, rate, seed, step, residual)
 
 
 class FusedDropout(nn.Module):
     """Dropout layer with its own seed and a step counter in device memory that every training call advances, in a
-    captured graph as well.  The counter is a buffer: a restored checkpoint continues the mask sequence."""
+    captured graph as well.  The counter is a buffer: a restored checkpoint continues the mask sequence.
+
+    A call inside a backward pass is a recomputation (activation checkpointing): it takes the step of the call it repeats and
+    leaves the counter alone.  Each training call draws one number from PyTorch's CPU generator to be known by; where that
+    number does not tell (``preserve_rng_state=False``, a generator seeded alike for several forward passes that wait
+    for their backward pass, more than ``REMEMBERED`` calls in between) the recomputation raises."""
 
     def __init__(self, rate: float, seed: int):
         super().__init__()
@@ -109,11 +125,32 @@ class FusedDropout(nn.Module):
             raise ValueError(f"FusedDropout: rate must lie in [0, 1], got {rate}")
         self.rate, self.seed = float(rate), int(seed)
         self.register_buffer("step", torch.zeros(1, dtype=torch.int64))
+        self._steps = OrderedDict()               # number of the call -> [its step, recomputed already]; step None: several calls
+
+    def __getstate__(self):
+        return {**self.__dict__, "_steps": OrderedDict()}
+
+    def _remember(self, call: int, used: torch.Tensor) -> None:
+        known = self._steps.pop(call, None)
+        # a call of the same number that still waits for its backward pass, or that never had one: which is meant?
+        self._steps[call] = [used if known is None or known[1] else None, False]
+        if len(self._steps) > REMEMBERED:
+            self._steps.popitem(last=False)
 
     def forward(self, x, residual=None):              # noqa: D102
         if not self.training or self.rate == 0.0:
             return x if residual is None else x + residual
-        y = dropout(x, self.rate, self.seed, self.step, residual)
+        call = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
+        if torch._C._current_graph_task_id() != -1:   # inside a backward pass
+            known = self._steps.get(call)
+            if known is None or known[0] is None:
+                raise RuntimeError("FusedDropout: called inside a backward pass, but not as the recomputation of one known forward pass; "
+                                   "activation checkpointing needs preserve_rng_state=True, or ops.dropout.dropout with a step of its own")
+            known[1] = True
+            return _dropout(x, self.rate, self.seed, known[0], residual)
+        used = torch.empty_like(self.step)
+        y = _dropout(x, self.rate, self.seed, self.step, residual, used)
+        self._remember(call, used)
         with torch.no_grad():
             self.step.add_(1)
         return y
