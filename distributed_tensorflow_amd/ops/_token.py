@@ -7,6 +7,7 @@ that captured it, so neither two streams nor two graphs ever share one.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -27,10 +28,19 @@ def at_most(what: str, n: int, most: int) -> None:
 
 
 def same_device(what: str, first: torch.Tensor, *others) -> None:
+    """Operands of one device; on a GPU none with a forward-mode tangent, which a kernel would drop without a word."""
     dev = first.device
     for t in others:
         if t is not None and t.device != dev:
             raise ValueError(f"{what}: tensors on different devices: {dev} vs {t.device}")
+    if forward_ad._current_level >= 0 and dev.type != "cpu":
+        refuse_tangents(what, first, *others)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: no forward-mode derivative on the GPU (CPU tensors have one)")
 
 
 def rows_2d(t: torch.Tensor, cols: int):
