@@ -43,6 +43,15 @@ def refuse_tangents(what: str, *tensors) -> None:
             raise NotImplementedError(f"{what}: no forward-mode derivative on the GPU (CPU tensors have one)")
 
 
+def in_one_type(x: torch.Tensor, residual):
+    """Under autocast a branch comes in autocast's type and the residual stream in float32: both in the wider type, as in
+    ``x + residual``."""
+    if residual is not None and residual.dtype != x.dtype and torch.is_autocast_enabled(x.device.type):
+        wide = torch.promote_types(x.dtype, residual.dtype)
+        return x.to(wide), residual.to(wide)
+    return x, residual
+
+
 def rows_2d(t: torch.Tensor, cols: int):
     """``t`` (last axis of ``cols`` elements) as rows and the distance between them; a copy only where no such view exists."""
     if t.is_contiguous():

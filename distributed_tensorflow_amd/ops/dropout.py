@@ -27,7 +27,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, reference
-from ._token import dtype_code, launch, same_device
+from ._token import dtype_code, in_one_type, launch, same_device
 
 _protos_done = False
 REMEMBERED = 1024          # calls of a FusedDropout whose step is kept for a recomputation
@@ -97,6 +97,7 @@ class _Dropout(torch.autograd.Function):
 
 
 def _dropout(x, rate, seed, step, residual, used=None):
+    x, residual = in_one_type(x, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, rate, seed, step, used)
     return dropout_apply(x, rate, seed, step, residual, used)
@@ -104,7 +105,8 @@ def _dropout(x, rate, seed, step, residual, used=None):
 
 def dropout(x: torch.Tensor, rate: float, seed: int, step: Union[int, torch.Tensor] = 0,
             residual: Optional[torch.Tensor] = None, training: bool = True) -> torch.Tensor:
-    """``[residual +] dropout(x)``; without ``training`` nothing is dropped."""
+    """``[residual +] dropout(x)``; without ``training`` nothing is dropped.  Under autocast a residual of another type than
+    ``x`` makes the result of the wider one."""
     if not training:
         return x if residual is None else x + residual
     return _dropout(x, rate, seed, step, residual)

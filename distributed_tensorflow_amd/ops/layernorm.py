@@ -23,7 +23,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, reference
-from ._token import at_most, dtype_code, launch, rows_2d, same_device
+from ._token import at_most, dtype_code, in_one_type, launch, rows_2d, same_device
 
 _protos_done = False
 
@@ -165,7 +165,9 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
-    """``y``, or ``(y, h)`` with a residual: layer normalisation of ``x [+ residual]`` over the last axis."""
+    """``y``, or ``(y, h)`` with a residual: layer normalisation of ``x [+ residual]`` over the last axis.  Under autocast a
+    residual of another type than ``x`` makes both results of the wider one."""
+    x, residual = in_one_type(x, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
         return _LayerNorm.apply(x, residual, weight, bias, eps)
     r = layer_norm_fwd(x, weight, bias, eps, residual)
