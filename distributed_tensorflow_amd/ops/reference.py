@@ -8,6 +8,7 @@ derives from it (``opt.minimize``, distributed.py:102).
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -201,6 +202,16 @@ def _vocab_labels(labels, vocab, ignore_index):
     return valid, lab
 
 
+def _float32_products(f):
+    """``f`` without autocast, which would run its products in a lower type."""
+    @functools.wraps(f)
+    def run(features, *args, **kw):
+        with torch.autocast(features.device.type, enabled=False):
+            return f(features, *args, **kw)
+    return run
+
+
+@_float32_products
 def vocab_xent(features, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
     """``(loss, rows, [hits, rows with a label])`` of softmax cross entropy on ``features @ weight.T + bias``; ``rows`` [4, N]:
     loss, logarithm of the sum of exponentials, largest logit, sum of exponentials relative to it."""
@@ -218,6 +229,7 @@ def vocab_xent(features, weight, labels, bias=None, ignore_index=-100, reduction
     return total, torch.stack((rows, lse, top, torch.exp(z - top[:, None]).sum(1))), counts
 
 
+@_float32_products
 def vocab_xent_bwd(features, weight, labels, bias, lse, counts, ignore_index=-100, reduction="mean", dloss=None):
     """``(dfeatures, dweight, dbias)``; dbias None without a bias."""
     x, w = features.float(), weight.float()
