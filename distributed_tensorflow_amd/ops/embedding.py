@@ -123,13 +123,19 @@ class ScaledEmbedding(nn.Embedding):
     """``nn.Embedding`` (same parameter and checkpoint name) whose output is multiplied by ``scale``."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: Optional[int] = None, **kw):
-        refused = set(kw) & {"max_norm", "scale_grad_by_freq", "sparse"}
-        if refused:
-            raise ValueError(f"ScaledEmbedding does not take {sorted(refused)}")
+        if kw.get("max_norm") is not None or kw.get("scale_grad_by_freq") or kw.get("sparse"):
+            raise ValueError("ScaledEmbedding does not take max_norm, scale_grad_by_freq or sparse")
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, **kw)
         if self.weight.dtype not in DTYPES:
             raise ValueError("ScaledEmbedding: float32 or bfloat16")
         self.scale = float(scale)
+
+    @classmethod
+    def from_pretrained(cls, embeddings, freeze: bool = True, padding_idx: Optional[int] = None, scale: float = 1.0, **kw):
+        """``nn.Embedding.from_pretrained`` with ``scale``."""
+        m = super().from_pretrained(embeddings, freeze, padding_idx, **kw)
+        m.scale = float(scale)
+        return m
 
     def forward(self, ids):                           # noqa: D102
         return embedding(ids, self.weight, self.scale, self.padding_idx)
