@@ -113,8 +113,9 @@ class _Embedding(torch.autograd.Function):
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * table[ids]``; tokens with id ``padding_idx`` give no gradient."""
-    if torch.is_grad_enabled() and table.requires_grad:
+    if padding_idx is not None and table.dim() == 2:
         _padding(padding_idx, table.shape[0])
+    if torch.is_grad_enabled() and table.requires_grad:
         return _Embedding.apply(ids, table, scale, padding_idx)
     return embedding_fwd(ids, table, scale)
 

@@ -22,3 +22,13 @@ def test_from_a_given_table(dev):
             em.ScaledEmbedding(9, 8, **bad)
         with pytest.raises(ValueError):
             em.ScaledEmbedding.from_pretrained(table, **bad)
+
+
+@pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_padding_index_outside_the_table_is_refused_with_and_without_gradients(grad, dev):
+    table, ids = torch.randn(9, 8, device=dev, requires_grad=grad), torch.zeros(2, dtype=torch.int64, device=dev)
+    for bad in (9, -10):
+        with pytest.raises(ValueError, match="padding_idx"):
+            em.embedding(ids, table, padding_idx=bad)
+    assert torch.equal(em.embedding(ids, table, padding_idx=-9), table[ids])
