@@ -178,6 +178,9 @@ class TorchModuleProgram:
 
     Has the interface the engines expect from ``MLPProgram`` (``run``, ``after_compute``,
     ``gs_inc``, ``fused``, ``read_log``) so that ``SyncReplicasEngine`` drives it unchanged.
+
+    The loss is the cross entropy of the module's logits, or what its method ``training_loss(inputs, labels)`` gives:
+    ``(loss, hits)``, as ``ops.vocab_xent.vocab_xent`` does for token models.
     """
 
     def __init__(self, module: nn.Module, device, images: torch.Tensor, labels: torch.Tensor, batch: int,
@@ -238,6 +241,8 @@ class TorchModuleProgram:
         self.post = False
         # classifier and loss on the framework's kernels where the module exposes its features (DTF_FUSED_HEAD=0: operators)
         self.fused_head = isinstance(self.module, ResNet) and os.environ.get("DTF_FUSED_HEAD", "1") != "0"
+        # a module that does not end in logits of a few classes brings its loss itself
+        self.own_loss = callable(getattr(self.module, "training_loss", None))
         # DTF_MODULE_GRAPH=1, one rank on a GPU: the whole step (forward, backward, optimizer) is captured into a
         # hipGraph after three eager steps and replayed; the host then only copies the next batch into the graph's
         # input buffers.  Opt-in: the ResNet-50 step is bound by the GPU (26.81 ms replayed, 26.97 ms eager on one stream; with the weight
@@ -427,6 +432,12 @@ class TorchModuleProgram:
             with torch.autocast(self.device.type, dtype=self.autocast, enabled=self.autocast is not None):
                 feat = self.module(x, features_only=True)
             loss, hits, _ = linear_xent(feat, self.module.fc.weight, self.module.fc.bias, y)
+            loss.backward()
+            self._last[0:1].copy_(loss.detach().reshape(1))
+            self._last[1:2].copy_(hits.reshape(1))
+        elif self.own_loss:
+            with torch.autocast(self.device.type, dtype=self.autocast, enabled=self.autocast is not None):
+                loss, hits = self.module.training_loss(x, y)
             loss.backward()
             self._last[0:1].copy_(loss.detach().reshape(1))
             self._last[1:2].copy_(hits.reshape(1))
