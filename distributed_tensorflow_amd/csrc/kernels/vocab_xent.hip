@@ -20,7 +20,7 @@
 // backward, 1400 TFLOP/s over the 8 N V D (a large library product: 1350); 4093 x 50001 x 1024 1.6 ms, where the epilogues of
 // the logits' launches are a third of their time; 777 x 10007 x 512 fp32 0.36 ms.  Few rows are bound by reading W (bf16, 16
 // rows at 65536 x 4096 forward and backward 0.56 ms: four passes over 0.54 GB), in fp32 from some 40 rows on by cutting and
-// multiplying planes (64 rows 1.21 ms: 113 TFLOP/s over the 8 N V D, a large fp32 library product 155).
+// multiplying planes (64 rows 1.24 ms: 111 TFLOP/s over the 8 N V D, a large fp32 library product 155).
 // Logits, statistics, loss and the column sums db are fp32; dz is rounded to the operands' type (bf16: half a step 2^-8 of
 // each element, the same rounding that any bf16 product of dz has).
 //

@@ -6,7 +6,8 @@ reciprocal of that keep probability.  The backward pass draws the same numbers a
 mask, and results do not depend on launch shapes, streams or devices: CPU tensors get the same mask.  ``residual`` adds
 the other branch of a residual block in the same pass.
 
-``seed`` belongs to a layer (give each layer of a model its own), ``step`` to a call: an integer, or a one-element int64
+``seed`` belongs to a layer (give each layer of a model its own; in a data-parallel run put the rank into it as well, or every
+replica draws the same mask for its own rows), ``step`` to a call: an integer, or a one-element int64
 tensor on x's device, whose value the kernel reads when it runs.  A captured graph that advances such a counter draws a
 new mask in every replay; the backward pass uses the value that its forward pass saw.
 

@@ -13,6 +13,8 @@ of about 1 GiB (or 16384 columns, whatever is more) backward, at any vocabulary 
   A label outside the vocabulary raises on the CPU; on the GPU, where raising would need a synchronisation, its row's
   loss (and with it the total) is NaN and the row gives no gradient.
 * ``reduction``: "mean" over the rows with a label (0 if there is none), "sum", or "none" (a loss per row).
+* a class is taken out by the bias -inf.  Infinities in features and weight follow float32 arithmetic at every size (a product
+  with -inf is -inf, 0 times an infinity is NaN, also in the features' gradient).
 * the hit count is the number of rows with a label whose label is the first maximum of the row.
 
 The reference's loss (distributed.py:81-87) is the ten-class case of this with logits kept; see ``classifier.py``.
