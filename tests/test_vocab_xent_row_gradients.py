@@ -84,3 +84,54 @@ def test_an_infinite_row_gradient_stays_in_its_row_of_dfeatures(n, v, dtype, dev
     others = torch.arange(n) != 6
     assert not torch.isfinite(dx[6]).any() and torch.equal(dx[others], clean[0][others])
     assert not torch.isfinite(dw).all() and not torch.isfinite(db).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
+def test_row_gradients_over_pieces_of_the_vocabulary(wdtype):
+    """40 000 columns at 16 416 tokens are more than one piece; dfeatures is scaled row by row behind the last one."""
+    n, v, d = 16416, 40001, 24
+    x, w, lab, b = (t.cuda() for t in draw(n, v, d, torch.bfloat16, wdtype))
+    r = vx.vocab_xent_fwd(x, w, lab, b, ignore_index=IGN, reduction="none")
+    s = vx.vocab_xent_fwd(x, w, lab, b, ignore_index=IGN, reduction="sum")
+    ones = vx.vocab_xent_bwd(s, x, w, lab, b)
+    for a, c in zip(vx.vocab_xent_bwd(r, x, w, lab, b, dloss=torch.full((n,), 1 / 8160, device="cuda")), ones):
+        c = c.double() / 8160
+        assert_within(a, c, (2 * half_step(a.dtype) + 2 * U32) * c.abs())
+    up = torch.randn(n, generator=torch.Generator().manual_seed(9)).cuda()
+    dx, dw, db = vx.vocab_xent_bwd(r, x, w, lab, b, dloss=up)
+    want = ones[0].double() * up.double()[:, None]                 # a row of dfeatures is linear in its gradient
+    assert_within(dx, want, (2 * half_step(dx.dtype) + 4 * U32) * want.abs())
+    g = torch.where(lab != IGN, up, 0.0).double()
+    z = x.double() @ w.to(torch.bfloat16).double().t()[:, :64] + b.double()[:64]
+    p = torch.exp(z - r.lse.double()[:, None]) - (lab[:, None] == torch.arange(64, device="cuda")).double()
+    size = (p * g[:, None]).abs()
+    # p off by less than 1e-4 of itself (sums of 24 and 40 001 terms), then dz and X rounded to bfloat16
+    bound = (2 * half_step(torch.bfloat16) + 1e-4) * (size.t() @ x.double().abs()) + half_step(dw.dtype) * dw[:64].double().abs()
+    assert_within(dw[:64], (p * g[:, None]).t() @ x.double(), bound)
+    assert_within(db[:64], (p * g[:, None]).sum(0), 1e-4 * size.sum(0))
+
+
+@pytest.mark.gpu
+def test_row_gradients_in_replayed_graphs():
+    x, w, lab, b = (t.cuda() for t in draw(300, 1111, 128, torch.bfloat16))
+    up = torch.rand(300, device="cuda")
+
+    def step():
+        r = vx.vocab_xent_fwd(x, w, lab, b, reduction="none")
+        return (r.loss_rows, *vx.vocab_xent_bwd(r, x, w, lab, b, dloss=up))
+    step()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for k in range(3):
+        up.copy_(torch.randn(300, generator=torch.Generator().manual_seed(k)) * 10.0 ** k)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for _, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(want, out))
